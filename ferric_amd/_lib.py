@@ -88,6 +88,10 @@ class Row(ctypes.Structure):
     ]
 
 
+class KvMove(ctypes.Structure):
+    _fields_ = [("src_page", ctypes.c_uint32), ("dst_page", ctypes.c_uint32), ("slots", ctypes.c_uint32)]
+
+
 _u16p = ctypes.POINTER(ctypes.c_uint16)
 _u32p = ctypes.POINTER(ctypes.c_uint32)
 _u64p = ctypes.POINTER(ctypes.c_uint64)
@@ -109,6 +113,7 @@ SIGNATURES = [
     ("fh_read_kv_page", _st, [_vp, _u32, _u32, _u32, _u16p, _u64]),
     ("fh_write_kv_page", _st, [_vp, _u32, _u32, _u32, _u16p, _u64]),
     ("fh_read_kv_cache", _st, [_vp, _u32, _u32, _u16p, _u64]),
+    ("fh_kv_copy_pages", _st, [_vp, _vp, _u32]),
     ("fh_execute_batch", _st, [_vp, _u64, ctypes.POINTER(Row), _u32, _u32p, _u32, _u32p]),
     ("fh_read_logits", _st, [_vp, _f32p, _u64]),
     ("fh_read_hidden", _st, [_vp, _u32, _u16p, _u64]),
@@ -145,6 +150,7 @@ SIGNATURES = [
     ("fh_op_swiglu", _st, [_vp, _vp, _vp, _u64, _vp, _vp]),
     ("fh_argmax_scratch_bytes", _u64, [_u32]),
     ("fh_op_argmax", _st, [_vp, _u32, _u32, _vp, _vp, _vp, _vp]),
+    ("fh_op_kv_copy_pages", _st, [_vp, _u32, _u64, _vp, _u32, _u32, _u32, _vp]),
     ("fh_op_synth_fill", _st, [_vp, _u64, _u64, ctypes.c_float, _vp]),
     ("fh_speculative_token_assembly", _st, [_u32p, _u32p, _u32, _u32, _u32p]),
     ("fh_verify_greedy_round", _st, [_u32p, _u32, _u32p, _u32, _u32p, _u32p, _u32p]),

@@ -5,6 +5,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "../../include/ferric_hip.h"
 #include "qk_head.hpp"
 
 namespace fh {
@@ -133,6 +134,17 @@ hipError_t launch_step_embed(const uint32_t* host, uint32_t* dev, uint32_t words
                              uint16_t* out, uint32_t rows, uint32_t hidden, uint32_t vocab, uint32_t* err,
                              hipStream_t s);
 hipError_t launch_copy_u16(const uint16_t* src, uint16_t* dst, uint64_t count, hipStream_t s);
+
+// Why a list of KV moves is refused (ops.hip), or nullptr; kNoMemory where it could not be checked.
+extern const char kNoMemory[];
+const char* kv_moves_refused(const fh_kv_move* moves, uint32_t count, uint32_t physical_pages);
+// KV page copies (k_pages.hip): move i copies the first slots[i * step] token
+// slots of page src[i * step] to page dst[i * step] (host arrays, words apart
+// by step) in each of cache_count caches cache_stride elements apart. No
+// destination occurs twice or is a source.
+hipError_t launch_kv_copy(uint16_t* caches, uint32_t cache_count, uint64_t cache_stride, const uint32_t* src,
+                          const uint32_t* dst, const uint32_t* slots, uint64_t step, uint32_t count, uint32_t kvh,
+                          hipStream_t s);
 
 // norms / activation
 hipError_t launch_rmsnorm(const uint16_t* x, const uint16_t* w, uint16_t* y, uint32_t rows, uint32_t width,

@@ -2,8 +2,11 @@
 // integer speculative-decoding helpers. Every entry point validates its
 // shapes on the host before launching, so a kernel never sees a geometry it
 // was not written for.
+#include <algorithm>
 #include <cstring>
 #include <mutex>
+#include <new>
+#include <vector>
 
 #include "../../include/ferric_hip.h"
 #include "kernels.hpp"
@@ -24,6 +27,43 @@ inline fh_status status_of(hipError_t e) {
 #define from_hip(expr) (static_cast<void>(hipGetLastError()), status_of(expr))
 
 }  // namespace
+
+namespace fh {
+
+const char kNoMemory[] = "no host memory to check the list";
+
+// Why a list of KV moves is refused, or nullptr. Independent copies need
+// destinations that occur once and are nobody's source.
+const char* kv_moves_refused(const fh_kv_move* moves, uint32_t count, uint32_t physical_pages) {
+  for (uint32_t i = 0; i < count; ++i) {
+    if (moves[i].src_page >= physical_pages || moves[i].dst_page >= physical_pages)
+      return "KV move: a page outside the pool";
+    if (moves[i].slots > 16) return "KV move: more than 16 slots";
+  }
+  static const char kTwice[] = "KV move: a destination occurs twice";
+  static const char kSource[] = "KV move: a destination is a source";
+  if (count <= 16) {  // a fork's few moves: no allocation
+    for (uint32_t i = 0; i < count; ++i)
+      for (uint32_t j = 0; j < count; ++j) {
+        if (i != j && moves[i].dst_page == moves[j].dst_page) return kTwice;
+        if (moves[i].dst_page == moves[j].src_page) return kSource;
+      }
+    return nullptr;
+  }
+  try {
+    std::vector<uint32_t> dst(count);
+    for (uint32_t i = 0; i < count; ++i) dst[i] = moves[i].dst_page;
+    std::sort(dst.begin(), dst.end());
+    if (std::adjacent_find(dst.begin(), dst.end()) != dst.end()) return kTwice;
+    for (uint32_t i = 0; i < count; ++i)
+      if (std::binary_search(dst.begin(), dst.end(), moves[i].src_page)) return kSource;
+  } catch (const std::bad_alloc&) {
+    return kNoMemory;
+  }
+  return nullptr;
+}
+
+}  // namespace fh
 
 extern "C" {
 
@@ -314,6 +354,23 @@ fh_status fh_op_argmax(const float* logits, uint32_t rows, uint32_t vocabulary, 
                        uint32_t* error_word, void* stream) {
   if (!logits || !scratch || !choices || rows == 0 || vocabulary == 0) return FH_ERR_INVALID_ARGUMENT;
   return from_hip(fh::launch_argmax(logits, rows, vocabulary, scratch, choices, error_word, as_stream(stream)));
+}
+
+fh_status fh_op_kv_copy_pages(uint16_t* caches, uint32_t cache_count, uint64_t cache_stride,
+                              const fh_kv_move* moves, uint32_t count, uint32_t kv_heads, uint32_t physical_pages,
+                              void* stream) {
+  if (!caches || (reinterpret_cast<uintptr_t>(caches) & 15u) || cache_count == 0 || cache_count > 65535u ||
+      (count && !moves) || kv_heads == 0 || kv_heads > 4096u || physical_pages == 0)
+    return FH_ERR_INVALID_ARGUMENT;
+  if (cache_count > 1 && (cache_stride % 8 || cache_stride < (uint64_t)physical_pages * 16 * kv_heads * 128))
+    return FH_ERR_INVALID_ARGUMENT;
+  if (const char* why = fh::kv_moves_refused(moves, count, physical_pages)) {
+    fh::set_thread_error(why);
+    return why == fh::kNoMemory ? FH_ERR_OUT_OF_MEMORY : FH_ERR_INVALID_ARGUMENT;
+  }
+  if (count == 0) return FH_OK;
+  return from_hip(fh::launch_kv_copy(caches, cache_count, cache_stride, &moves->src_page, &moves->dst_page,
+                                     &moves->slots, sizeof(fh_kv_move) / 4, count, kv_heads, as_stream(stream)));
 }
 
 fh_status fh_op_synth_fill(uint16_t* dst, uint64_t count, uint64_t tensor_seed, float scale, void* stream) {

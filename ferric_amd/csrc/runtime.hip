@@ -996,6 +996,24 @@ fh_status fh_write_kv_page(fh_ctx* ctx, uint32_t layer, uint32_t which, uint32_t
   return FH_OK;
 }
 
+fh_status fh_kv_copy_pages(fh_ctx* ctx, const fh_kv_move* moves, uint32_t count) {
+  if (!ctx || (count && !moves)) return fail(ctx, FH_ERR_INVALID_ARGUMENT, "null argument");
+  if (ctx->poisoned) return fail(ctx, FH_ERR_POISONED, "runtime poisoned by an earlier failure");
+  if (const char* why = fh::kv_moves_refused(moves, count, ctx->opt.physical_pages))
+    return fail(ctx, why == fh::kNoMemory ? FH_ERR_OUT_OF_MEMORY : FH_ERR_INVALID_ARGUMENT, why);
+  if (count == 0) return FH_OK;
+  (void)hipGetLastError();
+  // K and V of each layer lie one slab after the other.
+  const hipError_t e =
+      fh::launch_kv_copy(ctx->kv, 2 * ctx->md.layers, ctx->kv_slab_elems, &moves->src_page, &moves->dst_page,
+                         &moves->slots, sizeof(fh_kv_move) / 4, count, ctx->md.kv_heads, ctx->stream);
+  if (e != hipSuccess) {
+    ctx->poisoned = true;  // some of the moves may have been made
+    return hip_fail(ctx, e, "KV page copies");
+  }
+  return FH_OK;
+}
+
 // Attention blocks of a prefill chunk, cut from runs of rows of one sequence
 // at consecutive positions whose page lists extend one another (so a block's
 // last row's table serves every row of it), stored as first row | rows << 16.

@@ -33,6 +33,13 @@ class SequenceState:
     def pages(self) -> np.ndarray:
         return self._view
 
+    def replace_pages(self, pages: np.ndarray) -> None:
+        """Another page list of the same or another length, in an array of its
+        own: snapshots of the old list keep their entries."""
+        table = np.zeros_like(self._table)
+        table[: len(pages)] = pages
+        self._table, self._count, self._view = table, len(pages), table[: len(pages)]
+
     def append_page(self, page: int) -> None:
         self._table[self._count] = page
         self._count += 1
@@ -49,6 +56,8 @@ class PagePool:
         self.sequences: dict[int, SequenceState] = {}
         self._next_seq = 1
         self._next_batch = 1
+        self._shared: dict[int, int] = {}  # pages with more than one owner -> owners (fork)
+        self._moved_at = 1  # batches below this id were prepared before the pages moved
         # The last decode batch's page-list block: (sequence ids, page counts)
         # -> (tables, offsets, lengths). Equal ids and counts mean equal lists
         # (a sequence's pages are only appended; a released id never returns).
@@ -239,6 +248,8 @@ class PagePool:
         return states, sid, token, pos, group
 
     def commit(self, batch: PreparedBatch) -> None:
+        if batch.id < self._moved_at:
+            raise ValueError("the batch was prepared before compaction moved the pages")
         rows = batch.rows
         if isinstance(rows, PreparedRows):
             for s, p in zip(rows.sequence.tolist(), rows.position.tolist()):
@@ -256,8 +267,65 @@ class PagePool:
         st = self.sequences[sid]
         if length < 0 or (length + PAGE_TOKENS - 1) // PAGE_TOKENS > len(st.pages):
             raise ValueError("commit end outside the reserved pages")
+        if self._shared and any(int(p) in self._shared for p in st.pages[length // PAGE_TOKENS:]):
+            raise ValueError("commit end inside pages shared with another sequence")
         st.length = length
 
     def release(self, sid: int) -> None:
+        """Frees a sequence's pages; those it shares stay with their other owners."""
         st = self.sequences.pop(sid)
-        self.free.extend(int(p) for p in st.pages)
+        for p in st.pages:
+            p = int(p)
+            owners = self._shared.get(p, 1)
+            if owners > 2:
+                self._shared[p] = owners - 1
+            elif owners == 2:
+                del self._shared[p]
+            else:
+                self.free.append(p)
+
+    def fork(self, sid: int) -> tuple:
+        """A new sequence with the committed tokens of `sid`: (its id, moves).
+        The whole pages are shared; a partly filled last page gets a page of
+        the new sequence's own, filled by the one move returned, which the
+        caller hands to TpBatchRunner.copy_kv_pages before the next batch. The
+        moves of several forks may go in one call, but for a fork of a fork
+        whose move is not made yet: a page that is written and read is
+        refused. Raises MemoryError, changing nothing, without a free page."""
+        st = self.sequences[sid]
+        whole, rest = divmod(st.length, PAGE_TOKENS)
+        if rest and not self.free:
+            raise MemoryError("out of KV pages")
+        new = SequenceState(self._next_seq, self.limits.page_table_stride)
+        self._next_seq += 1
+        pages, moves = st.pages[:whole], []
+        if rest:
+            moves = [(int(st.pages[whole]), self.free.pop(), rest)]
+            pages = np.append(pages, np.uint32(moves[0][1]))
+        new.replace_pages(pages)
+        new.length = st.length
+        for p in st.pages[:whole]:
+            self._shared[int(p)] = self._shared.get(int(p), 1) + 1
+        self.sequences[new.sequence] = new
+        return new.sequence, moves
+
+    def compact(self) -> list:
+        """Moves the pages in use to the lowest page ids and returns the moves
+        for TpBatchRunner.copy_kv_pages: pages from the end of the pool go to
+        the holes below, the others stay. Every batch prepared before is to
+        be executed and committed first (commit refuses it afterwards)."""
+        used = sorted({int(p) for st in self.sequences.values() for p in st.pages})
+        n = len(used)
+        taken = set(used)
+        holes = [p for p in range(n) if p not in taken]
+        movers = [p for p in used if p >= n]
+        to = dict(zip(movers, holes))
+        if to:
+            for st in self.sequences.values():
+                if any(int(p) in to for p in st.pages):
+                    st.replace_pages(np.array([to.get(int(p), int(p)) for p in st.pages], dtype=np.uint32))
+            self._shared = {to.get(p, p): owners for p, owners in self._shared.items()}
+            self._decode_key = self._decode_tables = None
+            self._moved_at = self._next_batch
+        self.free = list(range(self.limits.physical_page_count - 1, n - 1, -1))
+        return [(src, dst, PAGE_TOKENS) for src, dst in to.items()]

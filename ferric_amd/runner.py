@@ -340,6 +340,18 @@ class TpBatchRunner:
                                         out.ctypes.data_as(ctypes.POINTER(ctypes.c_uint16)), n), self._ctx)
         return out
 
+    def copy_kv_pages(self, moves) -> None:
+        """Copies KV pages in every layer: moves as PagePool.fork and
+        PagePool.compact return them, [(source, destination, slots)]. Ordered
+        before the batches and readbacks after it; does not wait."""
+        m = np.asarray(moves)
+        if m.size == 0:
+            m = np.zeros((0, 3), dtype=np.uint32)
+        if m.ndim != 2 or m.shape[1] != 3 or m.dtype.kind not in "iu" or (m.size and (m.min() < 0 or m.max() > 0xFFFFFFFF)):
+            raise ValueError("KV moves are (source page, destination page, slots)")
+        m = np.ascontiguousarray(m, dtype=np.uint32)
+        check(self._lib.fh_kv_copy_pages(self._ctx, m.ctypes.data, len(m)), self._ctx)
+
     def read_kv_cache(self, layer: int, which: int) -> np.ndarray:
         """One layer's whole K (which = 0) or V (1) pool, [pages * 16 * kv_heads * 128] bf16."""
         n = self.limits.physical_page_count * PAGE_TOKENS * self.model["kv_heads"] * 128

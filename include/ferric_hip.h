@@ -143,6 +143,23 @@ fh_status fh_write_kv_page(fh_ctx* ctx, uint32_t layer, uint32_t which, uint32_t
  * elements must be that size): a parity readback, like fh_read_kv_page. */
 fh_status fh_read_kv_cache(fh_ctx* ctx, uint32_t layer, uint32_t which, uint16_t* out, uint64_t elements);
 
+/* A copy of the first `slots` token slots (0..16) of one physical KV page into another:
+ * a fork's partly filled last page, or a page that compaction moves. */
+typedef struct fh_kv_move {
+  uint32_t src_page;
+  uint32_t dst_page;
+  uint32_t slots;
+} fh_kv_move;
+
+/* Runs the moves in every layer's K and V pool, on the context's stream: batches and
+ * readbacks after the call see them, the call itself does not wait. The caller owns the
+ * pages as it does for batches (no batch prepared before a compaction is executed after
+ * it). Refused with FH_ERR_INVALID_ARGUMENT, copying nothing: a page outside the pool, more
+ * than 16 slots, a destination that occurs twice or is a source of any move. No counterpart
+ * in the reference, whose sealed-prefix copy-on-write (crates/ferric-engine/src/cache.rs:184)
+ * stays in its host model. */
+fh_status fh_kv_copy_pages(fh_ctx* ctx, const fh_kv_move* moves, uint32_t count);
+
 /* ---- the hot path ---- */
 
 /* Runs one forward step over the prepared rows and writes the greedy choice of
@@ -376,6 +393,16 @@ fh_status fh_op_swiglu(const uint16_t* gate, const uint16_t* up, uint16_t* out, 
 uint64_t fh_argmax_scratch_bytes(uint32_t rows);
 fh_status fh_op_argmax(const float* logits, uint32_t rows, uint32_t vocabulary, void* scratch,
                        uint32_t* choices, uint32_t* error_word, void* stream);
+
+/* KV page copies: for each of cache_count caches ([physical_pages][16][kv_heads][128] bf16,
+ * cache_stride elements apart; K and V of all layers, for instance) and each move,
+ * cache[dst_page][s] = cache[src_page][s] for s < slots; other slots keep their values.
+ * moves is host memory, read before the call returns. caches is 16-byte aligned;
+ * cache_stride (unused for one cache) is a multiple of 8 and at least one cache's elements;
+ * cache_count <= 65535. Refused as fh_kv_copy_pages. count = 0 does nothing. */
+fh_status fh_op_kv_copy_pages(uint16_t* caches, uint32_t cache_count, uint64_t cache_stride,
+                              const fh_kv_move* moves, uint32_t count, uint32_t kv_heads, uint32_t physical_pages,
+                              void* stream);
 
 /* Fills dst[0..count) with ferric_synth.h samples of (tensor_seed, index), scale from fh_synth_scale(). */
 fh_status fh_op_synth_fill(uint16_t* dst, uint64_t count, uint64_t tensor_seed, float scale, void* stream);
