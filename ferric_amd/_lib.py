@@ -130,6 +130,10 @@ SIGNATURES = [
     ("fh_op_embedding", _st, [_vp, _vp, _vp, _u32, _u32, _u32, _vp, _vp]),
     ("fh_op_rmsnorm", _st, [_vp, _vp, _vp, _u32, _u32, ctypes.c_float, _vp, _vp]),
     ("fh_op_gemm", _st, [_vp, _vp, _u32, _u32, _u32, _u32, _u32, _vp, _vp, _u32, _vp, _vp]),
+    ("fh_op_gemm_w4", _st, [_vp] * 4 + [_u32] * 6 + [_vp, _vp, _u32, _vp, _vp]),
+    ("fh_gemm_w4_default_splits", _u32, [_u32, _u32]),
+    ("fh_op_quantize_w4", _st, [_vp] * 3 + [_u32] * 3 + [_vp, _vp]),
+    ("fh_op_tile_weight_w4", _st, [_vp] * 6 + [_u32] * 4 + [_vp]),
     ("fh_gemm_default_splits", _u32, [_u32, _u32]),
     ("fh_gemm_block", _u32, [_u32] * 5),
     ("fh_prefill_attention_form", _u32, [ctypes.POINTER(ctypes.c_uint32)] * 2 + [_u32] * 3),

@@ -238,6 +238,20 @@ inline bool gemm_one_slab(uint32_t m, uint32_t n, uint32_t k) {
   return m > 64 && m <= kPanelRows && (uint64_t)n * k <= 8u << 20;
 }
 
+// 4-bit weights (k_gemm_w4.hip): m <= kMaxRows rows, n % 16 == 0, k % 128 == 0,
+// groups of 32, 64 or 128 columns; zeros may be null (8). The epilogues, x and
+// out are launch_gemm's.
+hipError_t launch_gemm_w4(const uint16_t* x_tiled, const uint32_t* w_tiled, const uint16_t* scales,
+                          const uint8_t* zeros, uint32_t m, uint32_t n, uint32_t k, uint32_t group, uint32_t epilogue,
+                          uint32_t splits, const uint16_t* residual, void* out, uint32_t ldo, uint32_t* err,
+                          hipStream_t s);
+uint32_t gemm_w4_default_splits(uint32_t n, uint32_t k);
+hipError_t launch_quantize_w4(const uint16_t* src, uint8_t* packed, uint16_t* scales, uint32_t n, uint32_t k,
+                              uint32_t group, uint32_t* err, hipStream_t s);
+hipError_t launch_tile_weight_w4(const uint8_t* packed, const uint16_t* scales, const uint8_t* zeros, uint32_t* w_tiled,
+                                 uint16_t* scales_tiled, uint8_t* zeros_tiled, uint32_t n, uint32_t k, uint32_t group,
+                                 uint32_t tile_mul, uint32_t tile_add, hipStream_t s);
+
 // attention
 // out: [rows][qh*128] row-major, or activation tile order when out_tiled.
 // Rows [0, rows) of a launch are rows row0 + [0, rows) of an output of

@@ -24,6 +24,12 @@ inline fh_status status_of(hipError_t e) {
 // Launchers report hipGetLastError(), which also returns an error left
 // behind by an unrelated earlier runtime call on this thread; clear it first
 // so that the status belongs to this launch.
+inline bool aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+inline bool w4_shape_ok(uint32_t n, uint32_t k, uint32_t group) {
+  return n != 0 && k != 0 && n % 16 == 0 && k % 128 == 0 && (group == 32 || group == 64 || group == 128);
+}
+
 #define from_hip(expr) (static_cast<void>(hipGetLastError()), status_of(expr))
 
 }  // namespace
@@ -127,6 +133,41 @@ fh_status fh_op_gemm(const uint16_t* x_tiled, const uint16_t* w_tiled, uint32_t 
   }
   return from_hip(fh::launch_gemm(x_tiled, w_tiled, m, n, k, epilogue, splits, residual, out, ldo, error_word,
                                             as_stream(stream)));
+}
+
+uint32_t fh_gemm_w4_default_splits(uint32_t n, uint32_t k) { return fh::gemm_w4_default_splits(n, k); }
+
+fh_status fh_op_gemm_w4(const uint16_t* x_tiled, const uint32_t* w_tiled, const uint16_t* scales_tiled,
+                        const uint8_t* zeros_tiled, uint32_t m, uint32_t n, uint32_t k, uint32_t group,
+                        uint32_t epilogue, uint32_t splits, const uint16_t* residual, void* out, uint32_t ldo,
+                        uint32_t* error_word, void* stream) {
+  if (!x_tiled || !w_tiled || !scales_tiled || !out || m == 0 || m > fh::kMaxRows || !w4_shape_ok(n, k, group))
+    return FH_ERR_INVALID_ARGUMENT;
+  if (!aligned(x_tiled, 16) || !aligned(w_tiled, 16) || !aligned(scales_tiled, 8) || !aligned(zeros_tiled, 4))
+    return FH_ERR_INVALID_ARGUMENT;
+  if (epilogue > FH_EPI_PARTIAL || splits == 0 || splits > k / 128 || splits > 65535u || (epilogue != FH_EPI_PARTIAL && splits != 1) ||
+      (epilogue == FH_EPI_RESIDUAL && !residual) || (epilogue == FH_EPI_SWIGLU ? n % 32 != 0 : ldo < n))
+    return FH_ERR_INVALID_ARGUMENT;
+  return from_hip(fh::launch_gemm_w4(x_tiled, w_tiled, scales_tiled, zeros_tiled, m, n, k, group, epilogue, splits,
+                                     residual, out, ldo, error_word, as_stream(stream)));
+}
+
+fh_status fh_op_quantize_w4(const uint16_t* src, uint8_t* packed, uint16_t* scales, uint32_t n, uint32_t k,
+                            uint32_t group, uint32_t* error_word, void* stream) {
+  if (!src || !packed || !scales || n == 0 || !w4_shape_ok(16, k, group) || (uint64_t)n * k > 1ull << 40 ||
+      !aligned(src, 16) || !aligned(packed, 4))
+    return FH_ERR_INVALID_ARGUMENT;
+  return from_hip(fh::launch_quantize_w4(src, packed, scales, n, k, group, error_word, as_stream(stream)));
+}
+
+fh_status fh_op_tile_weight_w4(const uint8_t* packed, const uint16_t* scales, const uint8_t* zeros,
+                               uint32_t* w_tiled, uint16_t* scales_tiled, uint8_t* zeros_tiled, uint32_t n, uint32_t k,
+                               uint32_t group, uint32_t part, void* stream) {
+  if (!packed || !scales || !w_tiled || !scales_tiled || (zeros && !zeros_tiled) || !w4_shape_ok(n, k, group) ||
+      (uint64_t)n * k > 1ull << 40 || part > 2 || !aligned(packed, 4) || !aligned(w_tiled, 16))
+    return FH_ERR_INVALID_ARGUMENT;
+  return from_hip(fh::launch_tile_weight_w4(packed, scales, zeros, w_tiled, scales_tiled, zeros_tiled, n, k, group,
+                                            part ? 2 : 1, part == 2 ? 1 : 0, as_stream(stream)));
 }
 
 uint32_t fh_gemm_block(uint32_t m, uint32_t n, uint32_t k, uint32_t epilogue, uint32_t fused_qkv) {

@@ -269,6 +269,37 @@ enum { FH_EPI_BF16 = 0, FH_EPI_RESIDUAL = 1, FH_EPI_SWIGLU = 2, FH_EPI_F32 = 3, 
 fh_status fh_op_gemm(const uint16_t* x_tiled, const uint16_t* w_tiled, uint32_t m, uint32_t n, uint32_t k,
                      uint32_t epilogue, uint32_t splits, const uint16_t* residual, void* out, uint32_t ldo,
                      uint32_t* error_word, void* stream);
+/* K1 projections with 4-bit weights and group scales, for decode batches (1 <= m <= 32):
+ * out = epilogue(x[m][k] . W[n][k]^T), W[n][k] = scale[n][k / group] * (q[n][k] - zero[n][k / group]),
+ * q in 0..15, zero 8 where zeros_tiled is NULL; FP32 accumulation on MFMA (the quantized
+ * weights enter it exactly). n % 16 == 0 (32 for FH_EPI_SWIGLU), k % 128 == 0, group 32, 64
+ * or 128. Epilogues, x_tiled, splits (<= k / 128 and 65535), residual, out, ldo and error_word as
+ * fh_op_gemm; only the first m rows of out are written. Operands in the order
+ * fh_op_tile_weight_w4 writes, w_tiled and x_tiled 16-byte, scales_tiled 8-byte and
+ * zeros_tiled 4-byte aligned. No counterpart in the reference, whose projections read bf16
+ * weights (gemm.rs:161/:605). */
+fh_status fh_op_gemm_w4(const uint16_t* x_tiled, const uint32_t* w_tiled, const uint16_t* scales_tiled,
+                        const uint8_t* zeros_tiled, uint32_t m, uint32_t n, uint32_t k, uint32_t group,
+                        uint32_t epilogue, uint32_t splits, const uint16_t* residual, void* out, uint32_t ldo,
+                        uint32_t* error_word, void* stream);
+/* Split-K factor for an n x k projection with 4-bit weights and FH_EPI_PARTIAL. */
+uint32_t fh_gemm_w4_default_splits(uint32_t n, uint32_t k);
+/* Rounds a row-major bf16 weight [n][k] to 4 bits per group (symmetric: no zero points):
+ * scale = bf16(max |w| / 7), q = 8 + clamp(rne(w / scale), -8, 7), 8 where the scale is 0.
+ * packed: [n][k / 2] bytes, even columns in the low half; scales: [n][k / group] bf16. k and
+ * group as fh_op_gemm_w4, n * k <= 2^40; src 16-byte, packed 4-byte aligned. error_word (may be
+ * NULL) receives the nonfinite bit where the weight holds a nonfinite value. */
+fh_status fh_op_quantize_w4(const uint16_t* src, uint8_t* packed, uint16_t* scales, uint32_t n, uint32_t k,
+                            uint32_t group, uint32_t* error_word, void* stream);
+/* Re-lays 4-bit weights (packed as above), their scales and zero points ([n][k / group]
+ * bytes; NULL: none, and zeros_tiled is not written) into the order fh_op_gemm_w4 reads:
+ * tiles of 16 rows x 128 columns of 1 KiB (n * k / 2 bytes in all), scales and zero points
+ * as [n / 16][k / group][16]. part 0: a whole operand. part 1 / 2: the gate / up half of
+ * an interleaved operand of 2 n rows for FH_EPI_SWIGLU (even / odd tile rows; call it for
+ * both). */
+fh_status fh_op_tile_weight_w4(const uint8_t* packed, const uint16_t* scales, const uint8_t* zeros,
+                               uint32_t* w_tiled, uint16_t* scales_tiled, uint8_t* zeros_tiled, uint32_t n, uint32_t k,
+                               uint32_t group, uint32_t part, void* stream);
 /* Split-K factor the runtime uses for an n x k projection. */
 uint32_t fh_gemm_default_splits(uint32_t n, uint32_t k);
 /* Output block of the compute-bound kernel that fh_op_gemm (or, with fused_qkv, a prefill

@@ -1,0 +1,293 @@
+"""4-bit projections on the GPU against the formula in 64 bits.
+
+Two kinds of inputs. Small whole activations and scales that are powers of two
+make every product and sum exact in FP32 (a group's sum of (128 + q) x stays
+below 143 * 128 * 8 < 2^18, an output below 2^24 steps of its last place), so
+the outputs have to be equal to the bit, whatever the order of the sums. Random
+ones are held to the roundings: FP32 sums of a group pass through partial sums
+of at most |sum (128 + q) x| over a run of its columns, at most one rounding of
+2^-24 of that per column and as many for the part taken off, then one per
+group; bf16 outputs add half a step, 2^-8 of the value."""
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+from tests import devutil as du  # noqa: E402
+import ferric_amd  # noqa: E402
+from ferric_amd import _lib  # noqa: E402
+from oracle import oracle as orc  # noqa: E402
+
+LIB = ferric_amd.load()
+BF16, RESIDUAL, SWIGLU, F32, PARTIAL = range(5)
+
+
+def widen(bits):
+    return (bits.astype(np.uint32) << 16).view(np.float32).astype(np.float64)
+
+
+def narrow(x):
+    """float64 to bf16 bits, one rounding (through FP32 only where that is exact)."""
+    x = np.asarray(x, np.float64)
+    f = x.astype(np.float32)
+    # Nearest FP32 with the sticky bit of what was lost: rounding it again is the one rounding to bf16.
+    b = f.view(np.uint32).copy()
+    off = np.abs(f.astype(np.float64)) > np.abs(x)
+    b[off] -= 1
+    b[(f.astype(np.float64) != x)] |= 1
+    return orc.f32_to_bf16(b.view(np.float32).reshape(-1)).reshape(x.shape)
+
+
+class Weight:
+    """Quantized values, scales and zero points on the host, and tiled on the device."""
+
+    def __init__(self, r, n, k, group, zeros, scales=None, half=False):
+        self.n, self.k, self.group = n, k, group
+        self.q = r.integers(0, 16, (n, k), dtype=np.uint8)
+        self.s = orc.f32_to_bf16((2.0 ** r.integers(-3, 4, n * (k // group))).astype(np.float32)) if scales is None else scales
+        self.s = self.s.reshape(n, k // group)
+        self.z = r.integers(0, 16, (n, k // group), dtype=np.uint8) if zeros else None
+        packed = self.q[:, 0::2] | (self.q[:, 1::2] << 4)
+        rows = 2 * n if half else n
+        d = dict(p=torch.from_numpy(packed.copy()).cuda(), s=du.to_dev(self.s))
+        d["z"] = torch.from_numpy(self.z).cuda() if zeros else None
+        self.dev = d
+        self.wt = torch.zeros(rows * k // 8, dtype=torch.int32, device="cuda")
+        self.st = torch.zeros(rows * (k // group), dtype=torch.int16, device="cuda")
+        self.zt = torch.zeros(rows * (k // group), dtype=torch.uint8, device="cuda") if zeros else None
+        if not half:
+            self.tile(self, 0)
+
+    def tile(self, into, part):
+        _lib.check(LIB.fh_op_tile_weight_w4(du.ptr(self.dev["p"]), du.ptr(self.dev["s"]), du.ptr(self.dev["z"]),
+                                            du.ptr(into.wt), du.ptr(into.st), du.ptr(into.zt), self.n, self.k, self.group,
+                                            part, du.stream()))
+
+    def exact(self):
+        z = self.z.astype(np.float64) if self.z is not None else np.full(self.s.shape, 8.0)
+        rep = lambda a: np.repeat(a, self.group, 1)  # noqa: E731
+        return rep(widen(self.s)) * (self.q.astype(np.float64) - rep(z))
+
+    def off(self, x):
+        """The bound on the FP32 error of x W^T (see above), x in 64 bits [m][k]."""
+        m, groups = x.shape[0], self.k // self.group
+        xg = x.reshape(m, groups, self.group)
+        zero = 128 + (self.z.astype(np.float64) if self.z is not None else 8.0)
+        runs = np.abs(np.cumsum(xg, 2)).max(2)  # [m][groups]
+        most = 2 * (143 + np.max(zero)) * runs + 16 * np.abs(xg).max(2) * np.sqrt(self.group)
+        return (2.0 ** -24) * (2 * self.group + 40) * (most @ np.abs(widen(self.s)).T)
+
+
+def activations(r, m, k, whole, junk=True):
+    """Row-major bits, and the tile order with rows past m full of NaN."""
+    x = r.integers(-8, 9, (m, k)).astype(np.float32) if whole else r.standard_normal((m, k)).astype(np.float32)
+    bits = orc.f32_to_bf16(x.reshape(-1)).reshape(m, k)
+    full = np.full((32, k), 0x7FC0 if junk else 0, np.uint16)
+    full[:m] = bits
+    return bits, du.to_dev(np.ascontiguousarray(full.reshape(2, 16, k // 32, 4, 8).transpose(2, 0, 3, 1, 4)).reshape(-1))
+
+
+def call(xt, w, m, n, epi, out, ldo, splits=1, residual=None, err=None, stream=None):
+    _lib.check(LIB.fh_op_gemm_w4(du.ptr(xt), du.ptr(w.wt), du.ptr(w.st), du.ptr(w.zt), m, n, w.k, w.group, epi, splits,
+                                 du.ptr(residual), du.ptr(out), ldo, du.ptr(err), stream or du.stream()))
+
+
+SHAPES = [(16, 128), (32, 256), (48, 384), (1040, 128), (4096, 1024), (64, 12288), (8192, 512), (16, 4096 + 128)]
+
+
+@pytest.mark.parametrize("n,k", SHAPES)
+@pytest.mark.parametrize("m", [1, 2, 8, 15, 16, 17, 32])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_whole_numbers_are_exact(n, k, m, group):
+    r = np.random.default_rng(n + k + m + group)
+    w = Weight(r, n, k, group, zeros=(n + m) % 2 == 1 or m == 8)
+    x, xt = activations(r, m, k, whole=True)
+    want = widen(x) @ w.exact().T
+    ldo = n + 5
+    out = torch.full(((m + 1) * ldo,), 7.5, dtype=torch.float32, device="cuda")
+    call(xt, w, m, n, F32, out, ldo)
+    got = du.to_host(out, np.float32).reshape(m + 1, ldo)
+    assert np.array_equal(got[:m, :n], want)
+    assert np.all(got[:m, n:] == 7.5) and np.all(got[m] == 7.5)  # nothing else is written
+    out = du.to_dev(np.full((m + 1) * n, 0x1234, np.uint16))
+    call(xt, w, m, n, BF16, out, n)
+    got = du.to_host(out, np.uint16).reshape(m + 1, n)
+    assert np.array_equal(got[:m], narrow(want)) and np.all(got[m] == 0x1234)
+
+
+@pytest.mark.parametrize("splits", [1, 2, 3, 5, 8])
+@pytest.mark.parametrize("m", [1, 20])
+def test_split_slabs_add_up_exactly(splits, m):
+    r = np.random.default_rng(splits)
+    n, k = 96, 1024
+    w = Weight(r, n, k, 64, True)
+    x, xt = activations(r, m, k, whole=True)
+    slab = 32 * n
+    out = torch.full((splits * slab + n,), 7.5, dtype=torch.float32, device="cuda")
+    call(xt, w, m, n, PARTIAL, out, n, splits)
+    got = du.to_host(out, np.float32)
+    assert np.all(got[splits * slab:] == 7.5)
+    slabs = got[:splits * slab].reshape(splits, 32, n)
+    assert np.array_equal(slabs[:, :m].astype(np.float64).sum(0), widen(x) @ w.exact().T)
+    assert np.all(slabs[:, m:] == 7.5)
+
+
+@pytest.mark.parametrize("m", [1, 9, 32])
+@pytest.mark.parametrize("alias", [False, True])
+def test_residual(m, alias):
+    r = np.random.default_rng(m)
+    n, k = 112, 384
+    w = Weight(r, n, k, 128, False)
+    x, xt = activations(r, m, k, whole=True)
+    res = orc.f32_to_bf16(r.integers(-99, 99, m * n).astype(np.float32))
+    dres = du.to_dev(res)
+    out = dres if alias else du.empty(m * n, np.uint16)
+    call(xt, w, m, n, RESIDUAL, out, n, residual=dres)
+    want = widen(x) @ w.exact().T + widen(res).reshape(m, n)
+    assert np.array_equal(du.to_host(out, np.uint16).reshape(m, n), narrow(want))
+
+
+@pytest.mark.parametrize("m", [1, 16, 17, 32])
+@pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, True)])
+def test_random_values_are_within_the_roundings(m, group, zeros):
+    r = np.random.default_rng(m + group)
+    n, k = 528, 2048
+    s = orc.f32_to_bf16((r.random(n * (k // group)) * 0.01 + 1e-3).astype(np.float32))
+    w = Weight(r, n, k, group, zeros, scales=s)
+    x, xt = activations(r, m, k, whole=False)
+    want, off = widen(x) @ w.exact().T, w.off(widen(x))
+    out = torch.zeros(m * n, dtype=torch.float32, device="cuda")
+    call(xt, w, m, n, F32, out, n)
+    got = du.to_host(out, np.float32).reshape(m, n).astype(np.float64)
+    assert np.all(np.abs(got - want) <= off)
+    # All roundings of a group taken as independent: 2^-25 * 136 / 4.6 * sqrt(128) = 1e-5 of the result's norm.
+    assert np.linalg.norm(got - want) <= 2e-5 * np.linalg.norm(want)
+    out = du.empty(m * n, np.uint16)
+    call(xt, w, m, n, BF16, out, n)
+    got = widen(du.to_host(out, np.uint16).reshape(m, n))
+    assert np.all(np.abs(got - want) <= off + 2.0 ** -8 * (np.abs(want) + off))
+
+
+@pytest.mark.parametrize("m", [1, 7, 16, 18, 32])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_swiglu_of_interleaved_halves_feeds_the_next_projection(m, zeros):
+    r = np.random.default_rng(m)
+    width, k, group = 256, 512, 64
+    scale = lambda a, b: orc.f32_to_bf16((r.random(a * b) * 0.01 + 2e-3).astype(np.float32))  # noqa: E731
+    gate = Weight(r, width, k, group, zeros, scales=scale(width, k // group), half=True)
+    up = Weight(r, width, k, group, zeros, scales=scale(width, k // group), half=True)
+    gate.tile(gate, 1)
+    up.tile(gate, 2)
+    x, xt = activations(r, m, k, whole=False)
+    out, err = du.to_dev(np.full(32 * width, 0x2222, np.uint16)), du.empty(1, np.uint32)
+    call(xt, gate, m, 2 * width, SWIGLU, out, width, err=err)
+    assert du.to_host(err, np.uint32)[0] == 0
+    tiled = du.to_host(out, np.uint16).reshape(width // 32, 2, 4, 16, 8).transpose(1, 3, 0, 2, 4).reshape(32, width)
+    assert np.all(tiled[m:] == 0x2222)
+    g, u = widen(x) @ gate.exact().T, widen(x) @ up.exact().T
+    # Half a step of bf16 for gate, up and the product, the FP32 sums before them; |d silu / dg| <= 1.1.
+    dg, du_ = gate.off(widen(x)) + 2.0 ** -8 * np.abs(g), up.off(widen(x)) + 2.0 ** -8 * np.abs(u)
+    silu = g / (1 + np.exp(-g))
+    want, off = silu * u, 1.1 * dg * (np.abs(u) + du_) + np.abs(silu) * du_
+    assert np.all(np.abs(widen(tiled[:m]) - want) <= (off + 2.0 ** -8 * (np.abs(want) + off)) * 1.001 + 1e-30)
+    # The tile-ordered output is the next projection's operand as it is.
+    down = Weight(r, 48, width, 128, zeros)
+    y = torch.zeros(m * 48, dtype=torch.float32, device="cuda")
+    call(out, down, m, 48, F32, y, 48)
+    a = widen(tiled[:m])
+    got = du.to_host(y, np.float32).reshape(m, 48)
+    assert np.all(np.abs(got - a @ down.exact().T) <= down.off(a))
+
+
+def test_swiglu_reports_nonfinite_rows_below_m_only():
+    r = np.random.default_rng(0)
+    w = Weight(r, 32, 128, 32, False)
+    _, xt = activations(r, 3, 128, whole=True)  # rows 3.. are NaN
+    out, err = du.empty(32 * 16, np.uint16), du.empty(1, np.uint32)
+    # 16 output columns are half a tile column of the next operand: the buffer holds 32 x 32.
+    out = du.empty(32 * 32, np.uint16)
+    call(xt, w, 3, 32, SWIGLU, out, 16, err=err)
+    assert du.to_host(err, np.uint32)[0] == 0
+    call(xt, w, 4, 32, SWIGLU, out, 16, err=err)
+    assert du.to_host(err, np.uint32)[0] == 1
+
+
+def test_extremes_of_weights_and_scales():
+    """All weights at the ends, scales at the ends of bf16, zero scales, zero points 0 and 15."""
+    r = np.random.default_rng(1)
+    n, k, m = 16, 256, 4
+    w = Weight(r, n, k, 32, True)
+    w.q[:8] = 0
+    w.q[8:] = 15
+    w.z[:, 0::2] = 0
+    w.z[:, 1::2] = 15
+    w.s[:] = 0x3F80
+    w.s[3] = 0
+    w.s[5] = 0x0080  # the smallest normal number
+    packed = w.q[:, 0::2] | (w.q[:, 1::2] << 4)
+    w.dev = dict(p=torch.from_numpy(packed.copy()).cuda(), s=du.to_dev(w.s), z=torch.from_numpy(w.z).cuda())
+    w.tile(w, 0)
+    x, xt = activations(r, m, k, whole=True)
+    out = torch.zeros(m * n, dtype=torch.float32, device="cuda")
+    call(xt, w, m, n, F32, out, n)
+    assert np.array_equal(du.to_host(out, np.float32).reshape(m, n), widen(x) @ w.exact().T)
+
+
+@pytest.mark.parametrize("n,k,group", [(1, 128, 32), (3, 256, 64), (33, 1152, 128), (1000, 384, 32)])
+def test_quantize_is_the_stated_rounding(n, k, group):
+    r = np.random.default_rng(n)
+    x = r.standard_normal((n, k)).astype(np.float32) * 0.02
+    x[0, :group] = 0  # a group of zeros
+    if n > 1:
+        x[1, :group] = 1e-39  # below the smallest normal number
+        x[-1, -group:] = r.integers(-7, 8, group)  # ties and ends
+    bits = orc.f32_to_bf16(x.reshape(-1))
+    w = widen(bits).astype(np.float32).reshape(n, k // group, group)
+    packed, scales = torch.zeros(n * k // 2 + 4, dtype=torch.uint8, device="cuda"), du.empty(n * (k // group) + 1, np.uint16)
+    err = du.empty(1, np.uint32)
+    src = du.to_dev(bits)
+    _lib.check(LIB.fh_op_quantize_w4(du.ptr(src), du.ptr(packed), du.ptr(scales), n, k, group, du.ptr(err), du.stream()))
+    s = orc.f32_to_bf16((np.abs(w).max(2) / np.float32(7)).reshape(-1))
+    got = du.to_host(scales, np.uint16)
+    assert np.array_equal(got[:-1], s) and got[-1] == 0 and du.to_host(err, np.uint32)[0] == 0
+    f = widen(s).astype(np.float32).reshape(n, -1, 1)
+    with np.errstate(divide="ignore", invalid="ignore"):
+        q = np.where(f > 0, np.clip(np.rint(w / f), -8, 7), 0).astype(np.int64) + 8
+    q = q.reshape(n, k).astype(np.uint8)
+    p = packed.cpu().numpy()
+    assert np.array_equal(p[:n * k // 2].reshape(n, k // 2), q[:, 0::2] | (q[:, 1::2] << 4)) and not p[n * k // 2:].any()
+
+
+def test_quantize_reports_nonfinite_weights():
+    for bad in (0x7F80, 0xFF80, 0x7FC0):
+        bits = np.full(128, 0x3F80, np.uint16)
+        bits[77] = bad
+        src, err = du.to_dev(bits), du.empty(1, np.uint32)
+        packed, scales = torch.zeros(64, dtype=torch.uint8, device="cuda"), du.empty(2, np.uint16)
+        _lib.check(LIB.fh_op_quantize_w4(du.ptr(src), du.ptr(packed), du.ptr(scales), 1, 128, 64, du.ptr(err), du.stream()))
+        assert du.to_host(err, np.uint32)[0] == 1
+
+
+def test_two_streams_and_a_replayed_graph():
+    r = np.random.default_rng(8)
+    n, k, m = 2048, 1024, 5
+    w = Weight(r, n, k, 128, True)
+    x, xt = activations(r, m, k, whole=True)
+    want = (widen(x) @ w.exact().T).astype(np.float32)
+    outs = [torch.zeros(m * n, dtype=torch.float32, device="cuda") for _ in range(3)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for s, o in zip(streams, outs):
+        call(xt, w, m, n, F32, o, n, stream=s.cuda_stream)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(xt, w, m, n, F32, outs[2], n)
+    for _ in range(3):
+        outs[2].fill_(-1)
+        graph.replay()
+        torch.cuda.synchronize()
+        for o in outs:
+            assert np.array_equal(du.to_host(o, np.float32).reshape(m, n), want)
