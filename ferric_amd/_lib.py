@@ -92,6 +92,10 @@ class KvMove(ctypes.Structure):
     _fields_ = [("src_page", ctypes.c_uint32), ("dst_page", ctypes.c_uint32), ("slots", ctypes.c_uint32)]
 
 
+class PrefixGroup(ctypes.Structure):
+    _fields_ = [("first_row", ctypes.c_uint32), ("rows", ctypes.c_uint32), ("prefix_pages", ctypes.c_uint32)]
+
+
 _u16p = ctypes.POINTER(ctypes.c_uint16)
 _u32p = ctypes.POINTER(ctypes.c_uint32)
 _u64p = ctypes.POINTER(ctypes.c_uint64)
@@ -151,6 +155,8 @@ SIGNATURES = [
     ("fh_op_qknorm_paged_attention", _st,
      [_vp, _u32] + [_vp] * 9 + [_u32, _vp] + [_u32] * 6 + [ctypes.c_float, _vp, _vp]),
     ("fh_op_paged_attention_noalloc", _st, [_vp] * 6 + [_u32] * 7 + [_vp, _vp]),
+    ("fh_prefix_attention_scratch_bytes", _u64, [_vp] + [_u32] * 5),
+    ("fh_op_prefix_attention", _st, [_vp] * 6 + [_u32, _vp, _u32, _vp, _u64] + [_u32] * 6 + [_vp, _vp]),
     ("fh_op_swiglu", _st, [_vp, _vp, _vp, _u64, _vp, _vp]),
     ("fh_argmax_scratch_bytes", _u64, [_u32]),
     ("fh_op_argmax", _st, [_vp, _u32, _u32, _vp, _vp, _vp, _vp]),

@@ -327,6 +327,20 @@ hipError_t launch_attention_prefill(uint32_t form, const uint16_t* q, const uint
                                     uint32_t rows, uint32_t qh, uint32_t kvh, uint32_t stride, uint32_t pages,
                                     uint32_t context, uint32_t* err, hipStream_t s);
 
+// Attention of rows that share prefixes (k_attention_prefix.hip). groups (host
+// memory): ascending, disjoint runs of rows [first_row, first_row + rows) of
+// the launch whose page tables agree in their first prefix_pages entries; rows
+// in no group share nothing. A row's position is at least 16 prefix_pages - 1.
+constexpr uint32_t kPrefixMaxGroups = 64;
+const char* prefix_groups_refused(const fh_prefix_group* groups, uint32_t ngroups, uint32_t rows, uint32_t context);
+uint64_t prefix_scratch_bytes(const fh_prefix_group* groups, uint32_t ngroups, uint32_t rows, uint32_t qh, uint32_t kvh,
+                              uint32_t context);
+hipError_t launch_prefix_attention(const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache,
+                                   const uint32_t* positions, const uint32_t* table, const fh_prefix_group* groups,
+                                   uint32_t ngroups, uint16_t* out, uint32_t out_tiled, void* scratch, uint32_t rows,
+                                   uint32_t qh, uint32_t kvh, uint32_t stride, uint32_t pages, uint32_t context,
+                                   uint32_t* err, hipStream_t s);
+
 // logits
 // With host_choices (coherent pinned memory), the choices and the error word
 // (at host_err) are also stored there, so the host reads them without a

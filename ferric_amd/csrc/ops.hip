@@ -26,6 +26,14 @@ inline fh_status status_of(hipError_t e) {
 // so that the status belongs to this launch.
 inline bool aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
+// Head counts of the attention kernels and sizes whose products fit the launch.
+inline bool prefix_shape_ok(uint32_t rows, uint32_t qh, uint32_t kvh, uint32_t context) {
+  if (rows == 0 || rows > 65535u || kvh == 0 || kvh > 4096u || qh % kvh != 0 || context == 0 || context > 1u << 30)
+    return false;
+  const uint32_t g = qh / kvh;
+  return g == 1 || g == 2 || g == 4 || g == 8;
+}
+
 inline bool w4_shape_ok(uint32_t n, uint32_t k, uint32_t group) {
   return n != 0 && k != 0 && n % 16 == 0 && k % 128 == 0 && (group == 32 || group == 64 || group == 128);
 }
@@ -65,6 +73,21 @@ const char* kv_moves_refused(const fh_kv_move* moves, uint32_t count, uint32_t p
       if (std::binary_search(dst.begin(), dst.end(), moves[i].src_page)) return kSource;
   } catch (const std::bad_alloc&) {
     return kNoMemory;
+  }
+  return nullptr;
+}
+
+// Why a batch's prefix groups are refused, or nullptr.
+const char* prefix_groups_refused(const fh_prefix_group* groups, uint32_t ngroups, uint32_t rows, uint32_t context) {
+  if (ngroups > kPrefixMaxGroups) return "prefix groups: more than 64";
+  if (ngroups && !groups) return "prefix groups: null";
+  uint64_t next = 0;
+  for (uint32_t i = 0; i < ngroups; ++i) {
+    const fh_prefix_group& g = groups[i];
+    if (g.rows == 0 || g.first_row < next || (uint64_t)g.first_row + g.rows > rows)
+      return "prefix groups: runs of rows have to be ascending, disjoint and within the batch";
+    if ((uint64_t)g.prefix_pages * 16 > context) return "prefix groups: a prefix beyond the context";
+    next = (uint64_t)g.first_row + g.rows;
   }
   return nullptr;
 }
@@ -381,6 +404,38 @@ fh_status fh_op_paged_attention(const uint16_t* q, const uint16_t* k_cache, cons
     e = fh::launch_attention_merge(part, positions, out, out_tiled, 0, rows, rows, query_heads, context_tokens,
                                    split_pages, error_word, s);
   return status_of(e);
+}
+
+uint64_t fh_prefix_attention_scratch_bytes(const fh_prefix_group* groups, uint32_t ngroups, uint32_t rows,
+                                           uint32_t query_heads, uint32_t kv_heads, uint32_t context_tokens) {
+  if (!prefix_shape_ok(rows, query_heads, kv_heads, context_tokens) ||
+      fh::prefix_groups_refused(groups, ngroups, rows, context_tokens))
+    return 0;
+  return fh::prefix_scratch_bytes(groups, ngroups, rows, query_heads, kv_heads, context_tokens);
+}
+
+fh_status fh_op_prefix_attention(const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache,
+                                 const uint32_t* positions, const uint32_t* page_table,
+                                 const fh_prefix_group* groups, uint32_t ngroups, uint16_t* out, uint32_t out_tiled,
+                                 void* scratch, uint64_t scratch_bytes, uint32_t rows, uint32_t query_heads,
+                                 uint32_t kv_heads, uint32_t stride, uint32_t physical_pages, uint32_t context_tokens,
+                                 uint32_t* error_word, void* stream) {
+  if (!q || !k_cache || !v_cache || !positions || !page_table || !out || !scratch || stride == 0 ||
+      physical_pages == 0 || (uint64_t)stride * 16 < context_tokens ||
+      !prefix_shape_ok(rows, query_heads, kv_heads, context_tokens) || !aligned(q, 16) || !aligned(k_cache, 16) ||
+      !aligned(v_cache, 16) || !aligned(out, 4) || !aligned(scratch, 16))
+    return FH_ERR_INVALID_ARGUMENT;
+  if (const char* why = fh::prefix_groups_refused(groups, ngroups, rows, context_tokens)) {
+    fh::set_thread_error(why);
+    return FH_ERR_INVALID_ARGUMENT;
+  }
+  if (scratch_bytes < fh::prefix_scratch_bytes(groups, ngroups, rows, query_heads, kv_heads, context_tokens)) {
+    fh::set_thread_error("fh_op_prefix_attention: the scratch is smaller than fh_prefix_attention_scratch_bytes()");
+    return FH_ERR_INVALID_ARGUMENT;
+  }
+  return from_hip(fh::launch_prefix_attention(q, k_cache, v_cache, positions, page_table, groups, ngroups, out,
+                                              out_tiled, scratch, rows, query_heads, kv_heads, stride, physical_pages,
+                                              context_tokens, error_word, as_stream(stream)));
 }
 
 fh_status fh_op_swiglu(const uint16_t* gate, const uint16_t* up, uint16_t* out, uint64_t elements,

@@ -413,6 +413,37 @@ fh_status fh_op_paged_attention_noalloc(const uint16_t* q, const uint16_t* k_cac
                                         uint32_t stride, uint32_t physical_pages, uint32_t context_tokens,
                                         uint32_t* error_word, void* stream);
 
+/* Rows [first_row, first_row + rows) of a batch whose page tables agree in their first
+ * prefix_pages entries: continuations of one prompt (forks), or rows of one sequence. */
+typedef struct fh_prefix_group {
+  uint32_t first_row;
+  uint32_t rows;
+  uint32_t prefix_pages;
+} fh_prefix_group;
+
+/* K4 for such batches: fh_op_paged_attention's result, with each group's prefix (16 x
+ * prefix_pages tokens) read once for all of its rows instead of once per row, and each row's
+ * other keys once for the row. groups is host memory, read before the call returns (a
+ * captured graph keeps them): 0..64 groups, ascending and disjoint; rows in no group share
+ * nothing. Any number of rows; several may belong to one sequence. Every row of a group has
+ * position >= 16 x prefix_pages - 1 (its prefix is all visible; ERR_POSITION in error_word
+ * and no output for the row otherwise), and its table's first prefix_pages entries are those
+ * of the group's first row (the page bit of error_word otherwise). q, out, out_tiled, tables
+ * and errors as fh_op_paged_attention; q and the caches 16-byte, out 4-byte aligned. scratch:
+ * fh_prefix_attention_scratch_bytes() of the same arguments, 16-byte aligned, for this call
+ * alone until it has run. Rows with one or several query heads per KV head (1, 2, 4, 8). FP32
+ * reassociation: the states of chunks of keys are merged, so the result differs from
+ * fh_op_paged_attention's in the order of its sums. No counterpart in the reference, whose
+ * decode attention reads every row's context (paged_decode.rs:222). */
+uint64_t fh_prefix_attention_scratch_bytes(const fh_prefix_group* groups, uint32_t ngroups, uint32_t rows,
+                                           uint32_t query_heads, uint32_t kv_heads, uint32_t context_tokens);
+fh_status fh_op_prefix_attention(const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache,
+                                 const uint32_t* positions, const uint32_t* page_table,
+                                 const fh_prefix_group* groups, uint32_t ngroups, uint16_t* out, uint32_t out_tiled,
+                                 void* scratch, uint64_t scratch_bytes, uint32_t rows, uint32_t query_heads,
+                                 uint32_t kv_heads, uint32_t stride, uint32_t physical_pages, uint32_t context_tokens,
+                                 uint32_t* error_word, void* stream);
+
 /* K6 SwiGLU as its own kernel: out = bf16(silu(g) * u), the stable-sigmoid form of
  * qwen3_swiglu_bf16_f32_v1 (device/qwen3-all-kernels-v1/src/swiglu.rs:62-120). */
 fh_status fh_op_swiglu(const uint16_t* gate, const uint16_t* up, uint16_t* out, uint64_t elements,
