@@ -25,6 +25,13 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
+constexpr int kKeys = 64;                      // keys per tile of a prefix chunk
+constexpr int kPages = kKeys / 16;             // pages per tile
+constexpr size_t kTileBytes = 16 * 2 * kKeys * 16;  // K or V, double-buffered
+constexpr uint32_t kOwnPages = 16;             // pages of a row's own keys the waves take at once
+constexpr uint32_t kMinChunk = 256;            // least tokens of a prefix chunk
+constexpr uint32_t kOwnUnits = 512;            // own keys are cut into about this many units
 // f32(0x3db504f3) (1/sqrt(128), paged_decode.rs:31-35) times log2 e.
 constexpr float kScoreScale = 0.08838834764831845f;
 constexpr float kLog2e = 1.44269504088896341f;
@@ -40,19 +47,16 @@ struct Groups {
 };
 
 // One state of nrows rows (consecutive from row0, sharing row0's table) over
-// keys [key0, key1), key0 a multiple of 16, for KV head h.
-template <int G, int WK>
-__device__ void attend(const uint16_t* __restrict__ q, const uint16_t* __restrict__ kc, const uint16_t* __restrict__ vc,
-                       const uint32_t* __restrict__ trow, uint32_t row0, uint32_t nrows, uint32_t key0, uint32_t key1,
-                       uint32_t h, uint32_t qh, uint32_t kvh, uint32_t pages, float* rec, uint32_t slots, uint32_t slot,
-                       uint32_t* err) {
-  constexpr int WQ = kWaves / WK;                // waves along the vectors
-  constexpr int kKeys = WK == 4 ? 128 : 64;      // keys per tile
+// keys [key0, key1), key0 a multiple of 16, for KV head h: the records of chunk
+// `slot`. WQ waves along the vectors (32 each), WK along the keys.
+template <int G, int WQ, int WK>
+__device__ __forceinline__ void attend_prefix(unsigned char* lds_raw, const uint16_t* __restrict__ q,
+                                              const uint16_t* __restrict__ kc, const uint16_t* __restrict__ vc,
+                                              const uint32_t* __restrict__ trow, uint32_t row0, uint32_t nrows,
+                                              uint32_t key0, uint32_t key1, uint32_t h, uint32_t qh, uint32_t kvh,
+                                              uint32_t pages, float* rec, uint32_t slots, uint32_t slot, uint32_t* err) {
   constexpr int kGroups = kKeys / 32 / WK;       // 32-key groups per wave and tile
-  constexpr int kPages = kKeys / 16;             // pages per tile
-  constexpr int kFetch = kPages / kWaves;        // of which each wave fetches this many
-  constexpr size_t kTileBytes = sizeof(u32x4) * 2 * kKeys * 16;
-  __shared__ __attribute__((aligned(16))) unsigned char lds_raw[2 * kTileBytes];
+  constexpr int kFetch = kPages / kWaves;        // pages of a tile each wave fetches
   auto& klds = *reinterpret_cast<u32x4(*)[2][kKeys][16]>(lds_raw);
   auto& vlds = *reinterpret_cast<u32x4(*)[2][kKeys][16]>(lds_raw + kTileBytes);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -103,8 +107,8 @@ __device__ void attend(const uint16_t* __restrict__ q, const uint16_t* __restric
   // j % G), dims 16 i + 8 (l / 32) .. + 7; vectors past the rows are zeros.
   const uint32_t c = lane & 31, hi = lane >> 5;
   const uint32_t rj = (32 * wq + c) / G, head = h * G + c % G;
-  const bool live = (uint32_t)(32 * wq / G) < nrows;  // a wave with no rows only fetches
-  const bool qvalid = rj < nrows;
+  const bool live = wq < WQ && (uint32_t)(32 * wq / G) < nrows;  // a wave with no rows only fetches
+  const bool qvalid = live && rj < nrows;
   u32x4 qv[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i)
@@ -237,7 +241,7 @@ __device__ void attend(const uint16_t* __restrict__ q, const uint16_t* __restric
   if constexpr (WK > 1) {
     // Waves wk > 0 hand their state over through the tiles' LDS.
     constexpr size_t kSlot = sizeof(f32x4) * 16 * 64 + sizeof(float) * 3 * 64;
-    static_assert(kSlot * WQ * (WK - 1) <= sizeof(lds_raw), "one slot per wave handing over");
+    static_assert(kSlot * WQ * (WK - 1) <= 2 * kTileBytes, "one slot per wave handing over");
     auto slot_acc = [&](int k) { return reinterpret_cast<f32x4*>(lds_raw + kSlot * (wq * (WK - 1) + k - 1)); };
     __syncthreads();  // every wave is done with the tiles
     if (live && wk > 0) {
@@ -290,82 +294,350 @@ __device__ void attend(const uint16_t* __restrict__ q, const uint16_t* __restric
   if (bad_page != 0 && lane == 0) raise_error(err, ERR_PAGE);
 }
 
-// Prefix items: (KV head, item).
-template <int G, int WK>
-__global__ __launch_bounds__(64 * kWaves, WK == 4 ? 1 : 2) void prefix_kernel(
-    const uint16_t* __restrict__ q, const uint16_t* __restrict__ kc, const uint16_t* __restrict__ vc,
-    const uint32_t* __restrict__ table, uint32_t qh, uint32_t kvh, uint32_t stride, uint32_t pages, float* rec,
-    uint32_t slots, uint32_t* err, Groups gs) {
-  const uint32_t h = blockIdx.x, item = blockIdx.y;
-  uint32_t gi = 0;
-  while (gi + 1 < gs.count && item >= gs.g[gi + 1].item0) ++gi;
-  const Group g = gs.g[gi];
-  const uint32_t blocks = (g.rows + gs.block_rows - 1) / gs.block_rows;
-  const uint32_t block = (item - g.item0) % blocks, chunk = (item - g.item0) / blocks;
-  const uint32_t first = block * gs.block_rows, nrows = min(gs.block_rows, g.rows - first);
-  const uint32_t key0 = chunk * gs.chunk, key1 = min(key0 + gs.chunk, g.prefix_tokens);
-  const uint32_t row0 = g.first_row + first;
-  const uint32_t* trow = table + (uint64_t)row0 * stride;
-  if (h == 0) {
-    // The rows of the block list the same pages here as the group's first row.
-    const uint32_t p0 = key0 / 16, np = (key1 - key0 + 15) / 16;
-    const uint32_t* lead = table + (uint64_t)g.first_row * stride;
-    bool differ = false;
-    for (uint32_t i = threadIdx.x; i < nrows * np; i += 64 * kWaves)
-      differ |= table[(uint64_t)(row0 + i / np) * stride + p0 + i % np] != lead[p0 + i % np];
-    if (differ) raise_error(err, ERR_PAGE);
-  }
-  attend<G, WK>(q, kc, vc, trow, row0, nrows, key0, key1, h, qh, kvh, pages, rec, slots, chunk, err);
-}
-
 __device__ __forceinline__ uint32_t prefix_of(const Groups& gs, uint32_t r) {
   for (uint32_t i = 0; i < gs.count; ++i)
     if (r - gs.g[i].first_row < gs.g[i].rows) return gs.g[i].prefix_tokens;
   return 0;
 }
 
-// A row's own keys [prefix, position], own_chunk at a time: (split, KV head, row).
-template <int G>
-__global__ __launch_bounds__(64 * kWaves, 1) void own_kernel(
-    const uint16_t* __restrict__ q, const uint16_t* __restrict__ kc, const uint16_t* __restrict__ vc,
-    const uint32_t* __restrict__ positions, const uint32_t* __restrict__ table, uint32_t qh, uint32_t kvh,
-    uint32_t stride, uint32_t pages, uint32_t context, uint32_t own_chunk, float* rec, uint32_t slots, uint32_t* err,
-    Groups gs) {
-  const uint32_t split = blockIdx.x, h = blockIdx.y, r = blockIdx.z;
-  const uint32_t pos = (uint32_t)__builtin_amdgcn_readfirstlane((int)positions[r]);
-  const uint32_t prefix = prefix_of(gs, r);
-  if (pos >= context || pos / 16 >= stride || pos + 1 < prefix) {
-    if (split == 0 && h == 0 && threadIdx.x == 0) raise_error(err, ERR_POSITION);
-    return;
-  }
-  const uint32_t key0 = prefix + split * own_chunk, key1 = min(key0 + own_chunk, pos + 1);
-  if (key0 >= key1) return;
-  attend<G, 4>(q, kc, vc, table + (uint64_t)r * stride, r, 1, key0, key1, h, qh, kvh, pages, rec, slots,
-               gs.prefix_slots + split, err);
+// Orders a wave's LDS accesses of the steps before and after it.
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// One wave per (row, query head): its records in ascending key order.
-__global__ __launch_bounds__(256) void prefix_merge_kernel(const float* __restrict__ rec,
+// What a workgroup that takes own keys needs of LDS.
+template <int G>
+struct OwnLds {
+  float sbuf[kWaves][64][G];  // scores, then probabilities: [token of the wave's four pages][head]
+  float stat[kWaves][2][G];
+  float acc[kWaves][G][128];
+  u32x4 ktile[kWaves][16][17];  // 272-byte rows keep the column reads conflict-free
+};
+
+// The state of row r over its keys of pages [page0, page1) of its table (keys
+// below ctx), for KV head h: G records at rec.
+template <int G>
+__device__ __forceinline__ void attend_own(unsigned char* lds_raw, const uint16_t* __restrict__ q,
+                                           const uint16_t* __restrict__ kc, const uint16_t* __restrict__ vc,
+                                           const uint32_t* __restrict__ trow, uint32_t r, uint32_t ctx, uint32_t page0,
+                                           uint32_t page1, uint32_t h, uint32_t qh, uint32_t kvh, uint32_t pages,
+                                           float* rec, uint32_t* err) {
+  constexpr uint32_t kWavePages = kOwnPages / kWaves;
+  auto& lds = *reinterpret_cast<OwnLds<G>*>(lds_raw);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t g16 = lane >> 4, r16 = lane & 15;
+  const float kNegInf = -__builtin_inff();
+  const float cs = kScoreScale * kLog2e;
+  float* sw = &lds.sbuf[wave][0][0];
+  bool bad = false;
+  uint32_t bad_page = 0;
+
+  // B operand: query head h G + r16 (zero for r16 >= G), dims 32 i + 8 g16 .. + 7.
+  u32x4 qv[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    qv[i] = r16 < G ? *reinterpret_cast<const u32x4*>(q + ((uint64_t)r * qh + h * G + r16) * 128 + 32 * i + 8 * g16)
+                    : u32x4{0u, 0u, 0u, 0u};
+  float m[G], l[G], acc[G][2];
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    m[g] = kNegInf;
+    l[g] = acc[g][0] = acc[g][1] = 0.f;
+  }
+  for (uint32_t at = page0; at < page1; at += kOwnPages) {
+    const uint32_t w0 = at + wave * kWavePages, np = w0 < page1 ? min(page1 - w0, kWavePages) : 0u;
+    if (np == 0) break;  // this wave has no more pages (no barrier in the loop)
+    uint32_t phys = lane < (int)np ? trow[w0 + lane] : 0u;
+    if (phys >= pages) {
+      bad_page = 1;
+      phys = 0;
+    }
+    auto phys_of = [&](uint32_t j) { return (uint32_t)__builtin_amdgcn_readlane((int)phys, (int)j); };
+    // Whole 256-byte token rows per load (lane: token 4 i + g16, dims 8 r16 .. + 7).
+    u32x4 kr[kWavePages][4];
+#pragma unroll
+    for (uint32_t u = 0; u < kWavePages; ++u)
+      if (u < np) {
+        const uint16_t* kp = kc + (((uint64_t)phys_of(u) * 16 + g16) * kvh + h) * 128 + 8 * r16;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) kr[u][i] = *reinterpret_cast<const u32x4*>(kp + (uint64_t)4 * i * kvh * 128);
+      }
+    uint32_t vd[kWavePages][16];
+#pragma unroll
+    for (uint32_t u = 0; u < kWavePages; ++u)
+      if (u < np) {
+        const uint32_t* vp = reinterpret_cast<const uint32_t*>(vc + (((uint64_t)phys_of(u) * 16) * kvh + h) * 128) + lane;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) vd[u][e] = vp[(uint64_t)e * kvh * 64];
+      }
+    // Scores: S^T = K Q^T a page at a time; lane: query r16, tokens 4 g16 + e.
+    float pm = kNegInf;
+#pragma unroll
+    for (uint32_t u = 0; u < kWavePages; ++u)
+      if (u < np) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) lds.ktile[wave][4 * i + g16][r16] = kr[u][i];
+        wave_fence();
+        f32x4 sacc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          sacc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, lds.ktile[wave][r16][g16 + 4 * i]),
+                                                        __builtin_bit_cast(bf16x8, qv[i]), sacc, 0, 0, 0);
+        wave_fence();
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool valid = (w0 + u) * 16 + 4 * g16 + e < ctx;
+          const float sv = valid ? sacc[e] * cs : kNegInf;
+          bad |= valid && !is_finite_f32(sv);
+          pm = fmaxf(pm, sv);
+          if (r16 < G) sw[(u * 16 + 4 * g16 + e) * G + r16] = sv;
+        }
+      }
+    pm = fmaxf(pm, __shfl_xor(pm, 16, 64));
+    pm = fmaxf(pm, __shfl_xor(pm, 32, 64));
+    float scale[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const float m_new = fmaxf(m[g], lane_bcast(pm, g));  // finite: a wave's pages hold a key
+      scale[g] = __builtin_amdgcn_exp2f(m[g] - m_new);
+      m[g] = m_new;
+    }
+    wave_fence();
+    // Probabilities in place, one token a lane; their sums.
+    if (lane < (int)(np * 16)) {
+#pragma unroll
+      for (int g = 0; g < G; ++g) sw[lane * G + g] = __builtin_amdgcn_exp2f(sw[lane * G + g] - m[g]);
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const float ps = lane < (int)(np * 16) ? sw[lane * G + g] : 0.f;
+      l[g] = l[g] * scale[g] + wave_sum(ps);
+      acc[g][0] *= scale[g];
+      acc[g][1] *= scale[g];
+    }
+    wave_fence();
+    // n += p v: lane owns dims 2 lane, 2 lane + 1.
+#pragma unroll
+    for (uint32_t u = 0; u < kWavePages; ++u)
+      if (u < np) {
+        const uint32_t valid = min(16u, ctx - (w0 + u) * 16);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const uint32_t v = (uint32_t)e < valid ? vd[u][e] : 0u;  // slots past the context may hold anything
+          const float v0 = lo_bf16(v), v1 = hi_bf16(v);
+#pragma unroll
+          for (int g = 0; g < G; ++g) {
+            const float p = sw[(u * 16 + e) * G + g];
+            acc[g][0] = __builtin_fmaf(p, v0, acc[g][0]);
+            acc[g][1] = __builtin_fmaf(p, v1, acc[g][1]);
+          }
+        }
+      }
+    wave_fence();
+  }
+  // The waves' states in wave order (a wave without pages has l = 0).
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    if (lane == 0) {
+      lds.stat[wave][0][g] = m[g];
+      lds.stat[wave][1][g] = l[g];
+    }
+    lds.acc[wave][g][2 * lane] = acc[g][0];
+    lds.acc[wave][g][2 * lane + 1] = acc[g][1];
+  }
+  __syncthreads();
+  for (int idx = threadIdx.x; idx < G * 128; idx += kThreads) {
+    const int g = idx >> 7, c = idx & 127;
+    float M = lds.stat[0][0][g];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) M = fmaxf(M, lds.stat[w][0][g]);
+    float n = 0.f, L = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float lw = lds.stat[w][1][g];
+      if (lw > 0.f) {
+        const float f = __builtin_amdgcn_exp2f(lds.stat[w][0][g] - M);
+        n += lds.acc[w][g][c] * f;
+        L += lw * f;
+      }
+    }
+    rec[g * kRecord + 4 + c] = n;
+    if (c == 0) {
+      rec[g * kRecord] = M;
+      rec[g * kRecord + 1] = L;
+      bad |= !(L > 0.f);
+    }
+  }
+  if (bad) raise_error(err, ERR_NONFINITE);
+  if (bad_page) raise_error(err, ERR_PAGE);
+}
+
+// Pages of row r's own keys; 0 where the row is not computed.
+__device__ __forceinline__ uint32_t own_pages(const uint32_t* positions, const Groups& gs, uint32_t r, uint32_t context,
+                                              uint32_t stride, bool& bad) {
+  const uint32_t pos = positions[r], prefix = prefix_of(gs, r);
+  if (pos >= context || pos / 16 >= stride || pos + 1 < prefix) {
+    bad = true;
+    return 0;
+  }
+  return (pos + 1 - prefix + 15) / 16;
+}
+
+// Workgroups [0, prefix_wgs): one chunk of a prefix for a block of rows and a
+// KV head. The others share the rows' own keys, cut into units of unit_pages
+// pages (a rule on the positions' total): every workgroup counts them for
+// itself, takes units own, own + own_wgs, ... of each KV head, and the first
+// one writes each row's first unit to `first` for the merge.
+template <int G, int WQ, int WK>
+__global__ __launch_bounds__(kThreads, 2) void prefix_kernel(
+    const uint16_t* __restrict__ q, const uint16_t* __restrict__ kc, const uint16_t* __restrict__ vc,
+    const uint32_t* __restrict__ positions, const uint32_t* __restrict__ table, uint32_t rows, uint32_t qh, uint32_t kvh,
+    uint32_t stride, uint32_t pages, uint32_t context, uint32_t prefix_wgs, uint32_t own_wgs, float* prefix_rec,
+    float* own_rec, uint32_t* first, uint32_t* err, Groups gs) {
+  __shared__ __attribute__((aligned(16))) unsigned char lds_raw[2 * kTileBytes];
+  static_assert(sizeof(OwnLds<G>) <= sizeof(lds_raw), "the own keys' part fits the tiles'");
+  if (blockIdx.x < prefix_wgs) {
+    const uint32_t h = blockIdx.x % kvh, item = blockIdx.x / kvh;
+    uint32_t gi = 0;
+    while (gi + 1 < gs.count && item >= gs.g[gi + 1].item0) ++gi;
+    const Group g = gs.g[gi];
+    const uint32_t blocks = (g.rows + gs.block_rows - 1) / gs.block_rows;
+    const uint32_t block = (item - g.item0) % blocks, chunk = (item - g.item0) / blocks;
+    const uint32_t in = block * gs.block_rows, nrows = min(gs.block_rows, g.rows - in);
+    const uint32_t key0 = chunk * gs.chunk, key1 = min(key0 + gs.chunk, g.prefix_tokens);
+    const uint32_t row0 = g.first_row + in;
+    if (h == 0) {
+      // The rows of the block list the same pages here as the group's first row.
+      const uint32_t p0 = key0 / 16, np = (key1 - key0 + 15) / 16;
+      const uint32_t* lead = table + (uint64_t)g.first_row * stride;
+      bool differ = false;
+      for (uint32_t i = threadIdx.x; i < nrows * np; i += kThreads)
+        differ |= table[(uint64_t)(row0 + i / np) * stride + p0 + i % np] != lead[p0 + i % np];
+      if (differ) raise_error(err, ERR_PAGE);
+    }
+    attend_prefix<G, WQ, WK>(lds_raw, q, kc, vc, table + (uint64_t)row0 * stride, row0, nrows, key0, key1, h, qh, kvh,
+                             pages, prefix_rec, gs.prefix_slots, chunk, err);
+    return;
+  }
+  const uint32_t own = blockIdx.x - prefix_wgs;
+  __shared__ uint32_t scan[kThreads];
+  __shared__ uint32_t wave_total[kWaves];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  // Sum over the workgroup (every thread gets it) and the sum up to this thread.
+  auto block_scan = [&](uint32_t v, uint32_t& total) {
+    uint32_t sum = v;
+#pragma unroll
+    for (int off = 1; off < 64; off *= 2) {
+      const uint32_t up = __shfl_up(sum, off, 64);
+      if (lane >= off) sum += up;
+    }
+    __syncthreads();
+    if (lane == 63) wave_total[wave] = sum;
+    __syncthreads();
+    total = 0;
+    for (int w = 0; w < kWaves; ++w) {
+      if (w < wave) sum += wave_total[w];
+      total += wave_total[w];
+    }
+    return sum;
+  };
+  uint64_t all = 0;
+  bool bad = false;
+  for (uint32_t r0 = 0; r0 < rows; r0 += kThreads) {
+    const uint32_t r = r0 + threadIdx.x;
+    uint32_t total;
+    block_scan(r < rows ? own_pages(positions, gs, r, context, stride, bad) : 0u, total);
+    all += total;
+  }
+  if (bad && own == 0) raise_error(err, ERR_POSITION);
+  // (The cap is beyond any row: one unit each.)
+  const uint32_t unit_pages =
+      (uint32_t)min((all * kvh / kOwnUnits + kOwnPages) / kOwnPages * kOwnPages, (uint64_t)1 << 24);
+  uint32_t base = 0;  // units of the rows before r0
+  uint32_t next = own;  // this workgroup's next (unit, head)
+  for (uint32_t r0 = 0; r0 < rows; r0 += kThreads) {
+    const uint32_t r = r0 + threadIdx.x;
+    const uint32_t mine = r < rows ? (own_pages(positions, gs, r, context, stride, bad) + unit_pages - 1) / unit_pages : 0u;
+    uint32_t total;
+    const uint32_t upto = block_scan(mine, total);
+    scan[threadIdx.x] = upto;
+    if (own == 0 && r < rows) {
+      first[r] = base + upto - mine;
+      if (r == rows - 1) first[rows] = base + upto;
+    }
+    __syncthreads();
+    for (; next < (base + total) * kvh; next += own_wgs) {
+      const uint32_t unit = next / kvh - base, h = next % kvh;
+      uint32_t lo = 0, hi = kThreads - 1;  // the first row whose units end after this one
+      while (lo < hi) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (scan[mid] > unit)
+          hi = mid;
+        else
+          lo = mid + 1;
+      }
+      const uint32_t row = __builtin_amdgcn_readfirstlane(r0 + lo);
+      const uint32_t before = lo ? scan[lo - 1] : 0u;
+      const uint32_t prefix = prefix_of(gs, row), ctx = __builtin_amdgcn_readfirstlane(positions[row]) + 1;
+      const uint32_t page0 = __builtin_amdgcn_readfirstlane(prefix / 16 + (unit - before) * unit_pages);
+      const uint32_t page1 = min(page0 + unit_pages, (ctx + 15) / 16);
+      attend_own<G>(lds_raw, q, kc, vc, table + (uint64_t)row * stride, row, ctx, page0, page1, h, qh, kvh, pages,
+                    own_rec + (uint64_t)next * G * kRecord, err);
+      __syncthreads();
+    }
+    base += total;
+    __syncthreads();
+  }
+}
+
+// One wave per (row, query head): its records in ascending key order, the
+// prefix's chunks and then its own units. Up to 64 records at a time: lane i
+// holds record i's weight, then every lane its two dims of eight records at once.
+__global__ __launch_bounds__(256) void prefix_merge_kernel(const float* __restrict__ prefix_rec,
+                                                          const float* __restrict__ own_rec,
+                                                          const uint32_t* __restrict__ first,
                                                           const uint32_t* __restrict__ positions,
                                                           uint16_t* __restrict__ out, uint32_t out_mtiles, uint32_t rows,
-                                                          uint32_t qh, uint32_t stride, uint32_t context,
-                                                          uint32_t own_chunk, uint32_t slots, uint32_t* err, Groups gs) {
+                                                          uint32_t qh, uint32_t kvh, uint32_t stride, uint32_t context,
+                                                          uint32_t* err, Groups gs) {
   const int lane = threadIdx.x & 63;
-  const uint32_t id = blockIdx.x * 4 + (threadIdx.x >> 6), r = id / qh, head = id % qh;
+  const uint32_t id = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = id / qh, head = id % qh;
   if (r >= rows) return;
   const uint32_t pos = positions[r], prefix = prefix_of(gs, r);
-  if (pos >= context || pos / 16 >= stride || pos + 1 < prefix) return;  // reported by the own keys' kernel
-  const uint32_t np = (prefix + gs.chunk - 1) / gs.chunk, no = (pos + 1 - prefix + own_chunk - 1) / own_chunk;
-  const float* p = rec + (uint64_t)id * slots * kRecord;
-  float M = -__builtin_inff(), L = 0.f, n0 = 0.f, n1 = 0.f;
-  for (uint32_t i = 0; i < np + no; ++i) {
-    const float* s = p + (uint64_t)(i < np ? i : gs.prefix_slots + i - np) * kRecord;
-    const float m = s[0], m_new = fmaxf(M, m);
-    const float a = __builtin_amdgcn_exp2f(M - m_new), b = __builtin_amdgcn_exp2f(m - m_new);
-    M = m_new;
-    L = L * a + s[1] * b;
-    n0 = n0 * a + s[4 + 2 * lane] * b;
-    n1 = n1 * a + s[5 + 2 * lane] * b;
+  if (pos >= context || pos / 16 >= stride || pos + 1 < prefix) return;  // reported by the own keys' part
+  const uint32_t u0 = first[r], np = (prefix + gs.chunk - 1) / gs.chunk, n = np + first[r + 1] - u0;
+  const uint32_t g = qh / kvh;
+  const float* pp = prefix_rec + (uint64_t)id * gs.prefix_slots * kRecord;
+  const float* po = own_rec + (((uint64_t)u0 * kvh + head / g) * g + head % g) * kRecord;
+  const uint64_t ostep = (uint64_t)kvh * g * kRecord;
+  auto record = [&](uint32_t i) { return i < np ? pp + (uint64_t)i * kRecord : po + (i - np) * ostep; };
+  float M = -__builtin_inff();
+  for (uint32_t i = lane; i < n; i += 64) M = fmaxf(M, record(i)[0]);
+  M = wave_max(M);
+  float L = 0.f, n0 = 0.f, n1 = 0.f;
+  for (uint32_t c0 = 0; c0 < n; c0 += 64) {
+    const uint32_t mine = min(c0 + lane, n - 1);
+    const float w = c0 + lane < n ? __builtin_amdgcn_exp2f(record(mine)[0] - M) : 0.f;
+    const float lw = w * record(mine)[1];
+    L += wave_sum(lw);
+    const uint32_t cn = min(64u, n - c0);
+    for (uint32_t s0 = 0; s0 < cn; s0 += 8) {
+      float a0[8], a1[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float2 v = *reinterpret_cast<const float2*>(record(c0 + min(s0 + u, cn - 1)) + 4 + 2 * lane);
+        a0[u] = v.x;
+        a1[u] = v.y;
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float f = s0 + u < cn ? lane_bcast(w, (int)(s0 + u)) : 0.f;
+        n0 = __builtin_fmaf(a0[u], f, n0);
+        n1 = __builtin_fmaf(a1[u], f, n1);
+      }
+    }
   }
   const uint32_t o0 = f32_to_bf16(n0 / L), o1 = f32_to_bf16(n1 / L);
   const uint32_t col = head * 128 + 2 * lane;
@@ -374,20 +646,15 @@ __global__ __launch_bounds__(256) void prefix_merge_kernel(const float* __restri
   if (!(L > 0.f) || ((o0 & 0x7f80u) == 0x7f80u) || ((o1 & 0x7f80u) == 0x7f80u)) raise_error(err, ERR_NONFINITE);
 }
 
-}  // namespace
-
-namespace {
-
-constexpr uint32_t kOwnChunk = 512;
-
 // The launch's work split: a rule on the groups, heads and lengths alone, so
 // that the scratch's size and the launch agree.
 struct PrefixPlan {
   Groups gs;
-  uint32_t items, form, own_splits, slots;
+  uint32_t items, form, own_wgs;
+  uint64_t prefix_floats, own_floats;  // of the records
 };
 
-PrefixPlan prefix_plan(const fh_prefix_group* groups, uint32_t ngroups, uint32_t qh, uint32_t kvh, uint32_t context) {
+PrefixPlan prefix_plan(const fh_prefix_group* groups, uint32_t ngroups, uint32_t rows, uint32_t qh, uint32_t kvh) {
   PrefixPlan p{};
   const uint32_t g = qh / kvh;
   uint32_t most = 0;
@@ -400,34 +667,32 @@ PrefixPlan prefix_plan(const fh_prefix_group* groups, uint32_t ngroups, uint32_t
   const uint64_t vectors = (uint64_t)most * g;
   p.form = vectors > 64 ? 1 : vectors > 32 ? 2 : 4;
   p.gs.block_rows = 128 / p.form / g;
-  // About one workgroup per CU over the prefixes, at least two tiles each.
+  // Two workgroups per CU over the prefixes, of at least kMinChunk tokens.
   uint64_t tokens = 0;
   for (uint32_t i = 0; i < p.gs.count; ++i)
     tokens += (uint64_t)p.gs.g[i].prefix_tokens * ((p.gs.g[i].rows + p.gs.block_rows - 1) / p.gs.block_rows) * kvh;
-  const uint32_t tile = p.form == 4 ? 128 : 64;
-  uint64_t chunk = (tokens / 256 + tile - 1) / tile * tile;
-  if (chunk < 2 * tile) chunk = 2 * tile;
+  uint64_t chunk = (tokens / 512 + kKeys - 1) / kKeys * kKeys;
+  if (chunk < kMinChunk) chunk = kMinChunk;
   p.gs.chunk = (uint32_t)chunk;
-  uint32_t at = 0;
   for (uint32_t i = 0; i < p.gs.count; ++i) {
     Group& to = p.gs.g[i];
     const uint32_t chunks = (to.prefix_tokens + p.gs.chunk - 1) / p.gs.chunk;
-    to.item0 = at;
-    at += chunks * ((to.rows + p.gs.block_rows - 1) / p.gs.block_rows);
+    to.item0 = p.items;
+    p.items += chunks * ((to.rows + p.gs.block_rows - 1) / p.gs.block_rows);
     if (chunks > p.gs.prefix_slots) p.gs.prefix_slots = chunks;
   }
-  p.items = at;
-  p.own_splits = (context + kOwnChunk - 1) / kOwnChunk;
-  p.slots = p.gs.prefix_slots + p.own_splits;
+  p.own_wgs = (uint64_t)rows * kvh < 256 ? 256 : 512;
+  p.prefix_floats = (uint64_t)rows * qh * p.gs.prefix_slots * kRecord;
+  // Units: a row's last one may be short, the others hold at least all / kOwnUnits pages and heads.
+  p.own_floats = ((uint64_t)kOwnUnits + kvh + (uint64_t)rows * kvh) * g * kRecord;
   return p;
 }
 
 }  // namespace
 
-uint64_t prefix_scratch_bytes(const fh_prefix_group* groups, uint32_t ngroups, uint32_t rows, uint32_t qh, uint32_t kvh,
-                              uint32_t context) {
-  const PrefixPlan p = prefix_plan(groups, ngroups, qh, kvh, context);
-  return (uint64_t)rows * qh * p.slots * kRecord * 4;
+uint64_t prefix_scratch_bytes(const fh_prefix_group* groups, uint32_t ngroups, uint32_t rows, uint32_t qh, uint32_t kvh) {
+  const PrefixPlan p = prefix_plan(groups, ngroups, rows, qh, kvh);
+  return (p.prefix_floats + p.own_floats + rows + 1) * 4;
 }
 
 hipError_t launch_prefix_attention(const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache,
@@ -435,24 +700,23 @@ hipError_t launch_prefix_attention(const uint16_t* q, const uint16_t* k_cache, c
                                    uint32_t ngroups, uint16_t* out, uint32_t out_tiled, void* scratch, uint32_t rows,
                                    uint32_t qh, uint32_t kvh, uint32_t stride, uint32_t pages, uint32_t context,
                                    uint32_t* err, hipStream_t s) {
-  const PrefixPlan p = prefix_plan(groups, ngroups, qh, kvh, context);
-  float* rec = reinterpret_cast<float*>(scratch);
-#define FH_PREFIX_WK(G_, WK_)                                                                                    \
-  hipLaunchKernelGGL((prefix_kernel<G_, WK_>), dim3(kvh, p.items), dim3(64 * kWaves), 0, s, q, k_cache, v_cache, \
-                     table, qh, kvh, stride, pages, rec, p.slots, err, p.gs)
-#define FH_PREFIX(G_)                                                                                            \
-  do {                                                                                                           \
-    if (p.items) {                                                                                               \
-      if (p.form == 1)                                                                                           \
-        FH_PREFIX_WK(G_, 1);                                                                                     \
-      else if (p.form == 2)                                                                                      \
-        FH_PREFIX_WK(G_, 2);                                                                                     \
-      else                                                                                                       \
-        FH_PREFIX_WK(G_, 4);                                                                                     \
-    }                                                                                                            \
-    hipLaunchKernelGGL((own_kernel<G_>), dim3(p.own_splits, kvh, rows), dim3(64 * kWaves), 0, s, q, k_cache,     \
-                       v_cache, positions, table, qh, kvh, stride, pages, context, kOwnChunk, rec, p.slots, err, \
-                       p.gs);                                                                                    \
+  const PrefixPlan p = prefix_plan(groups, ngroups, rows, qh, kvh);
+  float* prefix_rec = reinterpret_cast<float*>(scratch);
+  float* own_rec = prefix_rec + p.prefix_floats;
+  uint32_t* first = reinterpret_cast<uint32_t*>(own_rec + p.own_floats);
+  const uint32_t prefix_wgs = p.items * kvh;
+#define FH_PREFIX_FORM(G_, WQ_, WK_)                                                                               \
+  hipLaunchKernelGGL((prefix_kernel<G_, WQ_, WK_>), dim3(prefix_wgs + p.own_wgs), dim3(kThreads), 0, s, q, k_cache, \
+                     v_cache, positions, table, rows, qh, kvh, stride, pages, context, prefix_wgs, p.own_wgs,      \
+                     prefix_rec, own_rec, first, err, p.gs)
+#define FH_PREFIX(G_)              \
+  do {                             \
+    if (p.form == 1)               \
+      FH_PREFIX_FORM(G_, 4, 1);    \
+    else if (p.form == 2)          \
+      FH_PREFIX_FORM(G_, 2, 2);    \
+    else                           \
+      FH_PREFIX_FORM(G_, 1, 2);    \
   } while (0)
   switch (qh / kvh) {
     case 1: FH_PREFIX(1); break;
@@ -462,10 +726,12 @@ hipError_t launch_prefix_attention(const uint16_t* q, const uint16_t* k_cache, c
     default: return hipErrorInvalidValue;
   }
 #undef FH_PREFIX
-#undef FH_PREFIX_WK
+#undef FH_PREFIX_FORM
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
   const uint64_t waves = (uint64_t)rows * qh;
-  hipLaunchKernelGGL(prefix_merge_kernel, dim3((waves + 3) / 4), dim3(256), 0, s, rec, positions, out,
-                     out_tiled ? act_mtiles(rows) : 0u, rows, qh, stride, context, kOwnChunk, p.slots, err, p.gs);
+  hipLaunchKernelGGL(prefix_merge_kernel, dim3((waves + 3) / 4), dim3(256), 0, s, prefix_rec, own_rec, first, positions,
+                     out, out_tiled ? act_mtiles(rows) : 0u, rows, qh, kvh, stride, context, err, p.gs);
   return hipGetLastError();
 }
 

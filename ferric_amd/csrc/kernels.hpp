@@ -333,8 +333,7 @@ hipError_t launch_attention_prefill(uint32_t form, const uint16_t* q, const uint
 // in no group share nothing. A row's position is at least 16 prefix_pages - 1.
 constexpr uint32_t kPrefixMaxGroups = 64;
 const char* prefix_groups_refused(const fh_prefix_group* groups, uint32_t ngroups, uint32_t rows, uint32_t context);
-uint64_t prefix_scratch_bytes(const fh_prefix_group* groups, uint32_t ngroups, uint32_t rows, uint32_t qh, uint32_t kvh,
-                              uint32_t context);
+uint64_t prefix_scratch_bytes(const fh_prefix_group* groups, uint32_t ngroups, uint32_t rows, uint32_t qh, uint32_t kvh);
 hipError_t launch_prefix_attention(const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache,
                                    const uint32_t* positions, const uint32_t* table, const fh_prefix_group* groups,
                                    uint32_t ngroups, uint16_t* out, uint32_t out_tiled, void* scratch, uint32_t rows,

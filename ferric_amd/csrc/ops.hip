@@ -28,7 +28,7 @@ inline bool aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<u
 
 // Head counts of the attention kernels and sizes whose products fit the launch.
 inline bool prefix_shape_ok(uint32_t rows, uint32_t qh, uint32_t kvh, uint32_t context) {
-  if (rows == 0 || rows > 65535u || kvh == 0 || kvh > 4096u || qh % kvh != 0 || context == 0 || context > 1u << 30)
+  if (rows == 0 || rows > 65535u || kvh == 0 || kvh > 4096u || qh % kvh != 0 || context == 0 || context > 1u << 24)
     return false;
   const uint32_t g = qh / kvh;
   return g == 1 || g == 2 || g == 4 || g == 8;
@@ -411,7 +411,7 @@ uint64_t fh_prefix_attention_scratch_bytes(const fh_prefix_group* groups, uint32
   if (!prefix_shape_ok(rows, query_heads, kv_heads, context_tokens) ||
       fh::prefix_groups_refused(groups, ngroups, rows, context_tokens))
     return 0;
-  return fh::prefix_scratch_bytes(groups, ngroups, rows, query_heads, kv_heads, context_tokens);
+  return fh::prefix_scratch_bytes(groups, ngroups, rows, query_heads, kv_heads);
 }
 
 fh_status fh_op_prefix_attention(const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache,
@@ -429,7 +429,7 @@ fh_status fh_op_prefix_attention(const uint16_t* q, const uint16_t* k_cache, con
     fh::set_thread_error(why);
     return FH_ERR_INVALID_ARGUMENT;
   }
-  if (scratch_bytes < fh::prefix_scratch_bytes(groups, ngroups, rows, query_heads, kv_heads, context_tokens)) {
+  if (scratch_bytes < fh::prefix_scratch_bytes(groups, ngroups, rows, query_heads, kv_heads)) {
     fh::set_thread_error("fh_op_prefix_attention: the scratch is smaller than fh_prefix_attention_scratch_bytes()");
     return FH_ERR_INVALID_ARGUMENT;
   }

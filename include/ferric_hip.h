@@ -425,7 +425,7 @@ typedef struct fh_prefix_group {
  * prefix_pages tokens) read once for all of its rows instead of once per row, and each row's
  * other keys once for the row. groups is host memory, read before the call returns (a
  * captured graph keeps them): 0..64 groups, ascending and disjoint; rows in no group share
- * nothing. Any number of rows; several may belong to one sequence. Every row of a group has
+ * nothing. Up to 65535 rows and 2^24 context tokens; several rows may belong to one sequence. Every row of a group has
  * position >= 16 x prefix_pages - 1 (its prefix is all visible; ERR_POSITION in error_word
  * and no output for the row otherwise), and its table's first prefix_pages entries are those
  * of the group's first row (the page bit of error_word otherwise). q, out, out_tiled, tables
