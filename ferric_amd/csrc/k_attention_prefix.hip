@@ -7,9 +7,35 @@
 // out = bf16(n / l). Attention over a union of key sets is the merge of the
 // states over each: with (m_i, l_i, n_i) = (max s, sum e^(s - m_i), sum
 // e^(s - m_i) v), M = max m_i, out = sum n_i e^(m_i - M) / sum l_i e^(m_i - M).
-// A state covers a chunk of the prefix (for 128 / G, 64 / G or 32 / G rows at
-// once) or of a row's own keys; states are FP32 records in the scratch, merged
-// in ascending key order by a second launch.
+// A state covers a chunk of a prefix (for up to 128 query vectors of one KV head
+// at once) or a unit of a row's own keys; states are FP32 records in the
+// scratch, merged in ascending key order by a second launch.
+//
+// A wave owns 16 query vectors (vector j: row j / G, head j % G of the KV head)
+// and walks keys 32 or 64 at a time:
+//   S^T = K Q^T on v_mfma_f32_16x16x32_bf16, 16 keys a tile: lane l holds vector
+//   l % 16 and keys 4 (l / 16) + e (e = 0..3), so a vector's maximum is two
+//   exchanges between the four lane groups, and only when a tile's maximum
+//   exceeds the running one by more than 8 in the exponent of 2 does it move (the
+//   terms then reach at most 2^8: no precision is lost, and the accumulators are
+//   rescaled rarely). Each lane sums its own keys' terms until the end.
+//   O^T += V^T P^T on the same MFMA, 32 keys each: P is FP32 and enters as two
+//   bf16 terms, hi = bf16(p) and lo = bf16(p - hi) (within 2^-17 p of p). The B
+//   operand of two tiles is a lane's own eight terms, which fixes the order of the
+//   32 keys inside the MFMA; the V^T operand follows it with transposing LDS reads
+//   (ds_read_b64_tr_b16: 16 lanes read 4 keys x 16 dims, each lane gets one dim's
+//   4 keys).
+// LDS rows are 256 bytes (one token) with their 16-byte chunks permuted so that
+// the reads spread over the banks: K chunk c of key t at c ^ (t % 16), V chunk c
+// at c ^ 2 (t % 8). Slots that are no keys of the state are outside the loads'
+// buffer bounds and arrive as zeros, so what they hold never meets an MFMA.
+//
+// Two forms share the launch. Wide (prefix chunks of more than 16 vectors): the 8
+// waves share 64-key tiles of K and V, fetched global -> LDS directly, double-
+// buffered; 8 waves of vectors, or 4 with two of them sharing the tile's keys.
+// Narrow (own keys, and prefix chunks of up to 16 vectors): the waves take 32 keys
+// each, K straight into the A operand's registers (a token's 64-byte pieces), V
+// through 8 KiB of LDS of the wave's own; their states meet in LDS at the end.
 #include <type_traits>
 
 #include "common.hpp"
@@ -21,21 +47,19 @@ namespace {
 
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kWaves = 4;
+constexpr int kWaves = 8;
 constexpr int kThreads = 64 * kWaves;
-constexpr int kKeys = 64;                      // keys per tile of a prefix chunk
-constexpr int kPages = kKeys / 16;             // pages per tile
+constexpr int kKeys = 64;             // keys per tile of the wide form
+constexpr int kStep = 32 * kWaves;    // keys of the narrow form's waves at once
 constexpr size_t kTileBytes = 16 * 2 * kKeys * 16;  // K or V, double-buffered
-constexpr uint32_t kOwnPages = 16;             // pages of a row's own keys the waves take at once
-constexpr uint32_t kMinChunk = 256;            // least tokens of a prefix chunk
-constexpr uint32_t kOwnUnits = 512;            // own keys are cut into about this many units
+constexpr uint32_t kMinChunk = 256;   // least tokens of a prefix chunk
+constexpr uint32_t kOwnUnits = 256;   // own keys are cut into about this many units
+constexpr uint32_t kOwnWgs = 256;     // workgroups that take them
 // f32(0x3db504f3) (1/sqrt(128), paged_decode.rs:31-35) times log2 e.
-constexpr float kScoreScale = 0.08838834764831845f;
-constexpr float kLog2e = 1.44269504088896341f;
-constexpr uint32_t kRecord = 132;  // m, l, two unused, n[128]: 16-byte aligned
+constexpr float kScoreScale = 0.08838834764831845f * 1.44269504088896341f;
+constexpr uint32_t kRecord = 132;     // m, l, two unused, n[128]: 16-byte aligned
 
 struct Group {
   uint32_t first_row, rows, prefix_tokens;
@@ -46,153 +70,100 @@ struct Groups {
   Group g[kPrefixMaxGroups];
 };
 
-// One state of nrows rows (consecutive from row0, sharing row0's table) over
-// keys [key0, key1), key0 a multiple of 16, for KV head h: the records of chunk
-// `slot`. WQ waves along the vectors (32 each), WK along the keys.
-template <int G, int WQ, int WK>
-__device__ __forceinline__ void attend_prefix(unsigned char* lds_raw, const uint16_t* __restrict__ q,
-                                              const uint16_t* __restrict__ kc, const uint16_t* __restrict__ vc,
-                                              const uint32_t* __restrict__ trow, uint32_t row0, uint32_t nrows,
-                                              uint32_t key0, uint32_t key1, uint32_t h, uint32_t qh, uint32_t kvh,
-                                              uint32_t pages, float* rec, uint32_t slots, uint32_t slot, uint32_t* err) {
-  constexpr int kGroups = kKeys / 32 / WK;       // 32-key groups per wave and tile
-  constexpr int kFetch = kPages / kWaves;        // pages of a tile each wave fetches
-  auto& klds = *reinterpret_cast<u32x4(*)[2][kKeys][16]>(lds_raw);
-  auto& vlds = *reinterpret_cast<u32x4(*)[2][kKeys][16]>(lds_raw + kTileBytes);
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wq = wave / WK, wk = wave % WK;
-  const uint32_t page0 = key0 / 16, npages = (key1 - key0 + 15) / 16, tiles = (key1 - key0 + kKeys - 1) / kKeys;
+// What every state needs.
+struct Args {
+  const uint16_t *q, *kc, *vc;
+  uint32_t qh, kvh, pages;
+  uint32_t* err;
+};
 
-  auto table_chunk = [&](uint32_t first) { return first + lane < npages ? trow[page0 + first + lane] : 0u; };
-  uint32_t tab = table_chunk(0), tab_next = table_chunk(64);
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
 
-  const uint32_t token_bytes = kvh * 256;
-  uint32_t koff[4], voff[4];
+// Keeps a wave's LDS accesses before and after it in order.
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// Largest and sum over the four 16-lane groups that hold a vector's keys.
+__device__ __forceinline__ float group_max(float v) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, v);
+  const auto s = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+  const float w = fmaxf(__builtin_bit_cast(float, (uint32_t)s[0]), __builtin_bit_cast(float, (uint32_t)s[1]));
+  const uint32_t c = __builtin_bit_cast(uint32_t, w);
+  const auto t = __builtin_amdgcn_permlane32_swap(c, c, false, false);
+  return fmaxf(__builtin_bit_cast(float, (uint32_t)t[0]), __builtin_bit_cast(float, (uint32_t)t[1]));
+}
+__device__ __forceinline__ float group_sum(float v) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, v);
+  const auto s = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+  const float w = __builtin_bit_cast(float, (uint32_t)s[0]) + __builtin_bit_cast(float, (uint32_t)s[1]);
+  const uint32_t c = __builtin_bit_cast(uint32_t, w);
+  const auto t = __builtin_amdgcn_permlane32_swap(c, c, false, false);
+  return __builtin_bit_cast(float, (uint32_t)t[0]) + __builtin_bit_cast(float, (uint32_t)t[1]);
+}
+
+// A wave's running state of its 16 vectors.
+struct State {
+  float m, l, s_abs;  // of vector lane % 16: maximum, the lane's part of the sum, largest |score|
+  f32x4 acc[8];       // dims 16 d + 4 (lane / 16) + e
+
+  __device__ __forceinline__ void clear() {
+    m = -__builtin_inff();
+    l = s_abs = 0.f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t row = (4 * i + (lane >> 4)) * token_bytes;
-    koff[i] = row + (((lane & 15) ^ (4 * i + (lane >> 4))) & 15) * 16;
-    voff[i] = row + (((lane & 15) ^ ((lane >> 4) << 2)) & 15) * 16;
+    for (int d = 0; d < 8; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  uint32_t bad_page = 0;  // uniform
-  auto fetch = [&](uint32_t t, int buf) {
-#pragma unroll
-    for (int f = 0; f < kFetch; ++f) {
-      const uint32_t in_tile = wave + f * kWaves, pi = kPages * t + in_tile;
-      uint32_t page = (uint32_t)__builtin_amdgcn_readlane((int)tab, (int)(pi & 63u));
-      uint32_t valid = pi < npages ? min(16u, key1 - key0 - pi * 16) : 0u;  // keys of the page
-      if (page >= pages) {
-        bad_page |= valid;
-        page = 0;
-        valid = 0;
-      }
-      // Loads of tokens past the keys are out of bounds and return zeros.
-      const uint32_t bytes = valid * token_bytes;
-      const uint64_t base = ((uint64_t)page * 16 * kvh + h) * 128;
-      auto krs = __builtin_amdgcn_make_buffer_rsrc((void*)(kc + base), 0, bytes, 0x00020000);
-      auto vrs = __builtin_amdgcn_make_buffer_rsrc((void*)(vc + base), 0, bytes, 0x00020000);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            krs, (__attribute__((address_space(3))) void*)&klds[buf][16 * in_tile + 4 * i][0], 16, koff[i], 0, 0, 0);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            vrs, (__attribute__((address_space(3))) void*)&vlds[buf][16 * in_tile + 4 * i][0], 16, voff[i], 0, 0, 0);
-    }
-  };
-  fetch(0, 0);
 
-  // Query operand: lane l holds vector l % 32 of the wave (row j / G, head
-  // j % G), dims 16 i + 8 (l / 32) .. + 7; vectors past the rows are zeros.
-  const uint32_t c = lane & 31, hi = lane >> 5;
-  const uint32_t rj = (32 * wq + c) / G, head = h * G + c % G;
-  const bool live = wq < WQ && (uint32_t)(32 * wq / G) < nrows;  // a wave with no rows only fetches
-  const bool qvalid = live && rj < nrows;
-  u32x4 qv[8];
+  // Takes in T tiles of 16 scores: keys first + 16 t + 4 (lane / 16) + e below `end`. v_at(t, d): the V^T
+  // operand of tiles t, t + 1 (t even) for dims 16 d .. + 15.
+  template <int T, class V>
+  __device__ __forceinline__ void take(f32x4 (&s)[T], uint32_t first, uint32_t end, const V& v_at) {
+    const float kNegInf = -__builtin_inff();
+    const uint32_t at = first + 4 * ((threadIdx.x & 63) >> 4);
+    if (first + 16 * T > end) {
+      // Keys past the end: no term (and no part in the finiteness check).
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    qv[i] = qvalid ? *reinterpret_cast<const u32x4*>(q + ((uint64_t)(row0 + rj) * qh + head) * 128 + 16 * i + 8 * hi)
-                   : u32x4{0u, 0u, 0u, 0u};
-
-  const float kNegInf = -__builtin_inff();
-  const float cs = kScoreScale * kLog2e;
-  float m_run = kNegInf, l_run = 0.f, s_abs = 0.f;
-  f32x16 acc[4];  // output dims 32 d + 8 (e / 4) + 4 hi + e % 4 of vector c
+      for (int t = 0; t < T; ++t)
 #pragma unroll
-  for (int d = 0; d < 4; ++d)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
-
-  const u32x4* kl = &klds[0][c][0];
-  const uint32_t kx = c & 15;
-  const uint32_t tj = lane & 15, tkey = 4 * hi + (tj >> 2);
-  const uint32_t tchunk = ((lane >> 4) & 1) * 2 + ((tj & 3) >> 1), thalf = tj & 1;
-
-  auto compute = [&](uint32_t t) {
-    const int buf = t & 1;
-    const int own = kGroups * wk;  // this wave's first 32-key group of the tile
-    f32x16 s[kGroups];
-#pragma unroll
-    for (int kt = 0; kt < kGroups; ++kt) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) s[kt][e] = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const u32x4 ka = kl[(buf * kKeys + 32 * (own + kt)) * 16 + ((2 * i + hi) ^ kx)];
-        s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, ka),
-                                                        __builtin_bit_cast(bf16x8, qv[i]), s[kt], 0, 0, 0);
-      }
-    }
-    const uint32_t first = key0 + t * kKeys + 32 * own, at = first + 4 * hi;
-    if (first + 32 * kGroups > key1) {
-      // Keys past the chunk: no term (and no part in the finiteness check).
-#pragma unroll
-      for (int kt = 0; kt < kGroups; ++kt)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const bool ok = at + 32 * kt + 8 * (e >> 2) + (e & 3) < key1;
-          s_abs = fmaxf(s_abs, ok ? __builtin_fabsf(s[kt][e]) : 0.f);
-          s[kt][e] = ok ? s[kt][e] : kNegInf;
+        for (int e = 0; e < 4; ++e) {
+          const bool ok = at + 16 * t + e < end;
+          s_abs = fmaxf(s_abs, ok ? __builtin_fabsf(s[t][e]) : 0.f);
+          s[t][e] = ok ? s[t][e] : kNegInf;
         }
     } else {
 #pragma unroll
-      for (int kt = 0; kt < kGroups; ++kt)
+      for (int t = 0; t < T; ++t)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s_abs = fmaxf(s_abs, __builtin_fabsf(s[kt][e]));
+        for (int e = 0; e < 4; ++e) s_abs = fmaxf(s_abs, __builtin_fabsf(s[t][e]));
     }
-    float mt = kNegInf;
+    float top = kNegInf;
 #pragma unroll
-    for (int kt = 0; kt < kGroups; ++kt)
+    for (int t = 0; t < T; ++t)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[kt][e]);
-    {
-      const auto sw = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, mt), __builtin_bit_cast(uint32_t, mt),
-                                                       false, false);
-      mt = fmaxf(__builtin_bit_cast(float, (uint32_t)sw[0]), __builtin_bit_cast(float, (uint32_t)sw[1]));
+      for (int e = 0; e < 4; ++e) top = fmaxf(top, s[t][e]);
+    top = group_max(top);
+    // (No key at all so far: m and top both -inf, their difference NaN, no move.)
+    if (__builtin_amdgcn_ballot_w64((top - m) * kScoreScale > 8.f) != 0ull) {
+      const float m_new = fmaxf(m, top);
+      const float a = m == kNegInf ? 0.f : __builtin_amdgcn_exp2f((m - m_new) * kScoreScale);
+      m = m_new;
+      l *= a;
+#pragma unroll
+      for (int d = 0; d < 8; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[d][e] *= a;
     }
-    // A wave along the keys may meet no key in a tile (m_run and mt both
-    // -inf: their difference is NaN, no move).
-    if (__builtin_amdgcn_ballot_w64((mt - m_run) * cs > 8.f) != 0ull) {
-      const float m_new = fmaxf(m_run, mt);
-      const float alpha = m_run == kNegInf ? 0.f : __builtin_amdgcn_exp2f((m_run - m_new) * cs);
-      m_run = m_new;
-      l_run *= alpha;
+    const float mc = m == kNegInf ? 0.f : m * kScoreScale;
 #pragma unroll
-      for (int d = 0; d < 4; ++d)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) acc[d][e] *= alpha;
-    }
-    const float mc = m_run == kNegInf ? 0.f : m_run * cs;
-    float ps = 0.f;
-#pragma unroll
-    for (int g = 0; g < 2 * kGroups; ++g) {
+    for (int t = 0; t < T; t += 2) {
       float p[8];
       uint32_t ph[4], pl[4];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g >> 1][8 * (g & 1) + e], cs, -mc));
-        ps += p[e];
+        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t + (e >> 2)][e & 3], kScoreScale, -mc));
+        l += p[e];
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -202,276 +173,301 @@ __device__ __forceinline__ void attend_prefix(unsigned char* lds_raw, const uint
       const bf16x8 bh = __builtin_bit_cast(bf16x8, u32x4{ph[0], ph[1], ph[2], ph[3]});
       const bf16x8 bl = __builtin_bit_cast(bf16x8, u32x4{pl[0], pl[1], pl[2], pl[3]});
 #pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        u32x2 vq[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const uint32_t key = 32 * own + 16 * g + 8 * u + tkey;
-          const uint32_t chunk = (4 * d + tchunk) ^ ((tj >> 2) << 2);
-          auto* src = reinterpret_cast<u32x2*>(&vlds[buf][key][chunk]) + thalf;
-          vq[u] = __builtin_bit_cast(
-              u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)src));
-        }
-        const bf16x8 va = __builtin_bit_cast(bf16x8, u32x4{vq[0][0], vq[0][1], vq[1][0], vq[1][1]});
-        acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, bh, acc[d], 0, 0, 0);
-        acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, bl, acc[d], 0, 0, 0);
+      for (int d = 0; d < 8; ++d) {
+        const bf16x8 va = v_at(t, d);
+        acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, bh, acc[d], 0, 0, 0);
+        acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, bl, acc[d], 0, 0, 0);
       }
     }
-    l_run += ps;
+  }
+
+  // The vector's sum in every lane group.
+  __device__ __forceinline__ void finish() {
+    l = group_sum(l);
+    s_abs = group_max(s_abs);
+  }
+};
+
+// Transposing reads of V^T from LDS rows of tokens (u32x4[16] each): keys 16 t + 4 (lane / 16) + 0..3 of
+// tiles t and t + 1, dims 16 d .. + 15.
+__device__ __forceinline__ bf16x8 v_operand(const u32x4 (*rows)[16], int t, int d) {
+  const int lane = threadIdx.x & 63;
+  const uint32_t j = lane & 15, key = 4 * (lane >> 4) + (j >> 2);
+  u32x2 v[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const uint32_t k = 16 * (t + u) + key, c = (2 * d + ((j & 3) >> 1)) ^ (2 * (key & 7));
+    auto* src = reinterpret_cast<u32x2*>(const_cast<u32x4*>(&rows[k][c])) + (j & 1);
+    v[u] = __builtin_bit_cast(u32x2,
+                              __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)src));
+  }
+  return __builtin_bit_cast(bf16x8, u32x4{v[0][0], v[0][1], v[1][0], v[1][1]});
+}
+
+// Query operand: vector lane % 16 of the wave's 16 (vector `vec` of nrows rows), dims 32 i + 8 (lane / 16) .. + 7.
+template <int G>
+__device__ __forceinline__ void load_q(u32x4 (&qv)[4], const Args& a, uint32_t row0, uint32_t nrows, uint32_t vec,
+                                       uint32_t h) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    qv[i] = vec < nrows * G ? *reinterpret_cast<const u32x4*>(
+                                  a.q + ((uint64_t)(row0 + vec / G) * a.qh + h * G + vec % G) * 128 + 32 * i +
+                                  8 * (lane >> 4))
+                            : u32x4{0u, 0u, 0u, 0u};
+}
+
+// Record of (row, query head): m in the exponent of 2, l, n.
+__device__ __forceinline__ void store_record(float* r, const State& st, uint32_t* err) {
+  const int g16 = (threadIdx.x & 63) >> 4;
+  if (g16 == 0) {
+    r[0] = st.m * kScoreScale;
+    r[1] = st.l;
+  }
+#pragma unroll
+  for (int d = 0; d < 8; ++d) *reinterpret_cast<f32x4*>(r + 4 + 16 * d + 4 * g16) = st.acc[d];
+  if (!(st.l > 0.f) | !(st.s_abs < __builtin_inff())) raise_error(err, ERR_NONFINITE);
+}
+
+// A page of the table: its base for KV head h and the bytes of its first `valid` tokens (none where the page
+// is outside the pool).
+struct Page {
+  uint64_t base;
+  uint32_t bytes;
+};
+__device__ __forceinline__ Page page_of(const Args& a, uint32_t page, uint32_t valid, uint32_t h, uint32_t& bad) {
+  if (page >= a.pages) {
+    bad |= valid;
+    page = valid = 0;
+  }
+  return Page{((uint64_t)page * 16 * a.kvh + h) * 128, valid * a.kvh * 256};
+}
+
+// The wide form: nrows rows from row0 on (sharing trow's pages), keys [key0, key1) of KV head h, key0 a
+// multiple of 16. WK waves share a tile's keys, 8 / WK own the vectors. rec: record of (row 0, head 0), row
+// and head steps of `slots` records.
+template <int G, int WK>
+__device__ __forceinline__ void attend_wide(unsigned char* lds_raw, const Args& a, const uint32_t* __restrict__ trow,
+                                            uint32_t row0, uint32_t nrows, uint32_t key0, uint32_t key1, uint32_t h,
+                                            float* rec, uint32_t slots) {
+  constexpr int WQ = kWaves / WK, kTiles = kKeys / 16 / WK;  // 16-key tiles a wave takes of each 64
+  auto& klds = *reinterpret_cast<u32x4(*)[2][kKeys][16]>(lds_raw);
+  auto& vlds = *reinterpret_cast<u32x4(*)[2][kKeys][16]>(lds_raw + kTileBytes);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wq = wave % WQ, wk = wave / WQ;
+  const uint32_t page0 = key0 / 16, npages = (key1 - key0 + 15) / 16, tiles = (key1 - key0 + kKeys - 1) / kKeys;
+  // Page-table entries of 64 pages, one per lane, the next 64 requested ahead.
+  auto table_chunk = [&](uint32_t first) { return first + lane < npages ? trow[page0 + first + lane] : 0u; };
+  uint32_t tab = table_chunk(0), tab_next = table_chunk(64);
+  // Waves 0..3 copy K of the tile's pages 0..3, waves 4..7 V: four tokens per load (lane: token 4 i + lane /
+  // 16, LDS chunk lane % 16).
+  const int my_page = wave & 3;
+  const bool is_v = wave >= 4;
+  uint32_t off[4], bad_page = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t token = 4 * i + (lane >> 4), swizzle = is_v ? 2 * (token & 7) : token;
+    off[i] = token * a.kvh * 256 + (((lane & 15) ^ swizzle) & 15) * 16;
+  }
+  auto fetch = [&](uint32_t t, int buf) {
+    const uint32_t pi = 4 * t + my_page;
+    const uint32_t page = (uint32_t)__builtin_amdgcn_readlane((int)tab, (int)(pi & 63u));
+    const Page p = page_of(a, page, pi < npages ? min(16u, key1 - key0 - pi * 16) : 0u, h, bad_page);
+    auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)((is_v ? a.vc : a.kc) + p.base), 0, p.bytes, 0x00020000);
+    u32x4(*to)[16] = is_v ? vlds[buf] : klds[buf];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rsrc, (__attribute__((address_space(3))) void*)&to[16 * my_page + 4 * i][0], 16, off[i], 0, 0, 0);
   };
+  fetch(0, 0);
+  const uint32_t vec = 16 * wq + (lane & 15);
+  const bool live = (uint32_t)(16 * wq) < nrows * G;  // a wave with no vectors only fetches
+  u32x4 qv[4];
+  load_q<G>(qv, a, row0, nrows, vec, h);
+  State st;
+  st.clear();
   for (uint32_t t = 0; t < tiles; ++t) {
     __builtin_amdgcn_s_waitcnt(0 | (7u << 4) | (15u << 8));  // this wave's share of tile t is in LDS
     __syncthreads();  // everyone's is, and everyone is done with tile t - 1
     if (t + 1 < tiles) {
-      if ((t + 1) % (64 / kPages) == 0) {
+      if ((t + 1) % 16 == 0) {
         tab = tab_next;
-        tab_next = table_chunk(kPages * (t + 1) + 64);
+        tab_next = table_chunk(4 * (t + 1) + 64);
       }
       fetch(t + 1, (t + 1) & 1);
     }
-    if (live) compute(t);
+    if (!live) continue;
+    const int buf = t & 1, mine = kTiles * wk;
+    f32x4 s[kTiles];
+#pragma unroll
+    for (int u = 0; u < kTiles; ++u) {
+      s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const u32x4 ka = klds[buf][16 * (mine + u) + (lane & 15)][(4 * i + (lane >> 4)) ^ (lane & 15)];
+        s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, ka), __builtin_bit_cast(bf16x8, qv[i]),
+                                                       s[u], 0, 0, 0);
+      }
+    }
+    st.template take<kTiles>(s, key0 + t * kKeys + 16 * mine, key1,
+                             [&](int u, int d) { return v_operand(&vlds[buf][16 * mine], u, d); });
   }
-
-  float L = l_run;
-  {
-    const auto sw = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, L), __builtin_bit_cast(uint32_t, L),
-                                                     false, false);
-    L = __builtin_bit_cast(float, (uint32_t)sw[0]) + __builtin_bit_cast(float, (uint32_t)sw[1]);
-  }
-  if constexpr (WK > 1) {
-    // Waves wk > 0 hand their state over through the tiles' LDS.
-    constexpr size_t kSlot = sizeof(f32x4) * 16 * 64 + sizeof(float) * 3 * 64;
-    static_assert(kSlot * WQ * (WK - 1) <= 2 * kTileBytes, "one slot per wave handing over");
-    auto slot_acc = [&](int k) { return reinterpret_cast<f32x4*>(lds_raw + kSlot * (wq * (WK - 1) + k - 1)); };
+  st.finish();
+  if constexpr (WK == 2) {
+    // The waves of the tiles' second halves hand their state over through LDS.
+    struct Hand {
+      f32x4 acc[8][64];
+      float m[64], l[64], s_abs[64];
+    };
+    static_assert(sizeof(Hand) * WQ <= 2 * kTileBytes, "one slot per wave handing over");
+    Hand* hand = reinterpret_cast<Hand*>(lds_raw) + wq;
     __syncthreads();  // every wave is done with the tiles
-    if (live && wk > 0) {
-      f32x4* sa = slot_acc(wk);
-      float* sm = reinterpret_cast<float*>(sa + 16 * 64);
+    if (live && wk == 1) {
 #pragma unroll
-      for (int d = 0; d < 4; ++d)
-#pragma unroll
-        for (int e4 = 0; e4 < 4; ++e4)
-          sa[(4 * d + e4) * 64 + lane] =
-              f32x4{acc[d][4 * e4], acc[d][4 * e4 + 1], acc[d][4 * e4 + 2], acc[d][4 * e4 + 3]};
-      sm[lane] = m_run;
-      sm[64 + lane] = L;
-      sm[128 + lane] = s_abs;
+      for (int d = 0; d < 8; ++d) hand->acc[d][lane] = st.acc[d];
+      hand->m[lane] = st.m;
+      hand->l[lane] = st.l;
+      hand->s_abs[lane] = st.s_abs;
     }
     __syncthreads();
     if (live && wk == 0) {
+      const float kNegInf = -__builtin_inff();
+      const float m_new = fmaxf(st.m, hand->m[lane]);
+      const float fs = st.m == kNegInf ? 0.f : __builtin_amdgcn_exp2f((st.m - m_new) * kScoreScale);
+      const float fo = hand->m[lane] == kNegInf ? 0.f : __builtin_amdgcn_exp2f((hand->m[lane] - m_new) * kScoreScale);
+      st.m = m_new;
+      st.l = st.l * fs + hand->l[lane] * fo;
+      st.s_abs = fmaxf(st.s_abs, hand->s_abs[lane]);
 #pragma unroll
-      for (int k = 1; k < WK; ++k) {
-        const f32x4* sa = slot_acc(k);
-        const float* sm = reinterpret_cast<const float*>(sa + 16 * 64);
-        const float mo = sm[lane], lo = sm[64 + lane];
-        s_abs = fmaxf(s_abs, sm[128 + lane]);
-        const float m_new = fmaxf(m_run, mo);
-        const float fs = m_run == kNegInf ? 0.f : __builtin_amdgcn_exp2f((m_run - m_new) * cs);
-        const float fo = mo == kNegInf ? 0.f : __builtin_amdgcn_exp2f((mo - m_new) * cs);
-        m_run = m_new;
-        L = L * fs + lo * fo;
+      for (int d = 0; d < 8; ++d)
 #pragma unroll
-        for (int d = 0; d < 4; ++d)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) acc[d][e] = acc[d][e] * fs + sa[(4 * d + (e >> 2)) * 64 + lane][e & 3] * fo;
-      }
+        for (int e = 0; e < 4; ++e) st.acc[d][e] = st.acc[d][e] * fs + hand->acc[d][lane][e] * fo;
     }
   }
-  if (live && wk == 0 && qvalid) {
-    float* r = rec + (((uint64_t)(row0 + rj) * qh + head) * slots + slot) * kRecord;
-    if (hi == 0) {
-      r[0] = m_run * cs;  // in the exponent of 2
+  if (live && wk == 0 && vec < nrows * G)
+    store_record(rec + ((uint64_t)(vec / G) * a.qh + vec % G) * slots * kRecord, st, a.err);
+  if (bad_page != 0 && lane == 0) raise_error(a.err, ERR_PAGE);
+}
+
+// LDS of the narrow form: V of each wave's 32 keys, then the waves' states.
+struct NarrowState {
+  float acc[kWaves][16][128];
+};
+static_assert(sizeof(NarrowState) == 2 * kTileBytes, "the states of 8 waves fill the tiles' LDS");
+
+// The narrow form: as above for nrows * G <= 16 vectors. The record of vector v is rec + (v / G) * row_step +
+// (v % G) * head_step.
+template <int G>
+__device__ __forceinline__ void attend_narrow(unsigned char* lds_raw, const Args& a, const uint32_t* __restrict__ trow,
+                                              uint32_t row0, uint32_t nrows, uint32_t key0, uint32_t key1, uint32_t h,
+                                              float* rec, uint64_t row_step, uint64_t head_step) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  u32x4(*vlds)[16] = reinterpret_cast<u32x4(*)[16]>(lds_raw) + 32 * wave;
+  const uint32_t page0 = key0 / 16, npages = (key1 - key0 + 15) / 16, steps = (key1 - key0 + kStep - 1) / kStep;
+  // Table entries of this wave's two pages of 32 steps: lane 2 i + u holds page u of step i.
+  auto table_chunk = [&](uint32_t step) {
+    const uint32_t pi = (step + (lane >> 1)) * (kStep / 16) + 2 * wave + (lane & 1);
+    return pi < npages ? trow[page0 + pi] : 0u;
+  };
+  uint32_t tab = table_chunk(0), bad_page = 0;
+  u32x4 qv[4];
+  load_q<G>(qv, a, row0, nrows, lane & 15, h);
+  uint32_t koff, voff[4];
+  koff = (lane & 15) * a.kvh * 256 + 16 * (lane >> 4);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t token = 4 * i + (lane >> 4);
+    voff[i] = token * a.kvh * 256 + (((lane & 15) ^ (2 * (token & 7))) & 15) * 16;
+  }
+  State st;
+  st.clear();
+  for (uint32_t step = 0; step < steps; ++step) {
+    const uint32_t first = step * kStep + 32 * wave;  // key0-relative
+    if (first >= key1 - key0) break;  // no more keys for this wave (no barrier in the loop)
+    if (step != 0 && step % 32 == 0) tab = table_chunk(step);
+    // V first: the wait for K, whose registers the compiler tracks, then covers both kinds of loads.
+    u32x4 kr[2][4];
+    Page pg[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const uint32_t pi = first / 16 + u;
+      const uint32_t page = (uint32_t)__builtin_amdgcn_readlane((int)tab, (int)(2 * (step & 31u) + u));
+      pg[u] = page_of(a, page, pi < npages ? min(16u, key1 - key0 - pi * 16) : 0u, h, bad_page);
+      auto vrs = __builtin_amdgcn_make_buffer_rsrc((void*)(a.vc + pg[u].base), 0, pg[u].bytes, 0x00020000);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(vrs, (__attribute__((address_space(3))) void*)&vlds[16 * u + 4 * i][0],
+                                                 16, voff[i], 0, 0, 0);
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      auto krs = __builtin_amdgcn_make_buffer_rsrc((void*)(a.kc + pg[u].base), 0, pg[u].bytes, 0x00020000);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        kr[u][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(krs, koff, 64 * i, 0));
+    }
+    __builtin_amdgcn_s_waitcnt(0 | (7u << 4) | (15u << 8));
+    wave_fence();
+    f32x4 s[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kr[u][i]),
+                                                       __builtin_bit_cast(bf16x8, qv[i]), s[u], 0, 0, 0);
+    }
+    st.template take<2>(s, key0 + first, key1, [&](int u, int d) { return v_operand(vlds, u, d); });
+    // The next step's loads overwrite V: this step's reads of it are done.
+    __builtin_amdgcn_s_waitcnt(15u | (3u << 14) | (7u << 4) | (0u << 8));
+    wave_fence();
+  }
+  st.finish();
+  // The waves' states meet in LDS, the waves in order (one without keys has l = 0 and m = -inf).
+  __shared__ float wm[kWaves][16], wl[kWaves][16];
+  __syncthreads();  // every wave is done with its V
+  auto& all = *reinterpret_cast<NarrowState*>(lds_raw);
+  const uint32_t vec = lane & 15, nvec = nrows * G;
+  if (vec < nvec) {
+#pragma unroll
+    for (int d = 0; d < 8; ++d) *reinterpret_cast<f32x4*>(&all.acc[wave][vec][16 * d + 4 * (lane >> 4)]) = st.acc[d];
+    if (lane < 16) {
+      wm[wave][vec] = st.m * kScoreScale;
+      wl[wave][vec] = st.l;
+    }
+    if (st.l != st.l || !(st.s_abs < __builtin_inff())) raise_error(a.err, ERR_NONFINITE);
+  }
+  if (bad_page != 0 && lane == 0) raise_error(a.err, ERR_PAGE);
+  __syncthreads();
+  for (uint32_t idx = threadIdx.x; idx < nvec * 32; idx += kThreads) {
+    const uint32_t v = idx >> 5, c = idx & 31;  // four dims
+    float M = wm[0][v];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) M = fmaxf(M, wm[w][v]);
+    f32x4 n = f32x4{0.f, 0.f, 0.f, 0.f};
+    float L = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float f = wl[w][v] > 0.f ? __builtin_amdgcn_exp2f(wm[w][v] - M) : 0.f;
+      const f32x4 x = *reinterpret_cast<const f32x4*>(&all.acc[w][v][4 * c]);
+      L += wl[w][v] * f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) n[e] += x[e] * f;
+    }
+    float* r = rec + (v / G) * row_step + (v % G) * head_step;
+    *reinterpret_cast<f32x4*>(r + 4 + 4 * c) = n;
+    if (c == 0) {
+      r[0] = M;
       r[1] = L;
     }
-#pragma unroll
-    for (int d = 0; d < 4; ++d)
-#pragma unroll
-      for (int e4 = 0; e4 < 4; ++e4)
-        *reinterpret_cast<f32x4*>(r + 4 + 32 * d + 8 * e4 + 4 * hi) =
-            f32x4{acc[d][4 * e4], acc[d][4 * e4 + 1], acc[d][4 * e4 + 2], acc[d][4 * e4 + 3]};
-    if (!(L > 0.f) | !(s_abs < __builtin_inff())) raise_error(err, ERR_NONFINITE);
   }
-  if (bad_page != 0 && lane == 0) raise_error(err, ERR_PAGE);
 }
 
 __device__ __forceinline__ uint32_t prefix_of(const Groups& gs, uint32_t r) {
   for (uint32_t i = 0; i < gs.count; ++i)
     if (r - gs.g[i].first_row < gs.g[i].rows) return gs.g[i].prefix_tokens;
   return 0;
-}
-
-// Orders a wave's LDS accesses of the steps before and after it.
-__device__ __forceinline__ void wave_fence() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
-// What a workgroup that takes own keys needs of LDS.
-template <int G>
-struct OwnLds {
-  float sbuf[kWaves][64][G];  // scores, then probabilities: [token of the wave's four pages][head]
-  float stat[kWaves][2][G];
-  float acc[kWaves][G][128];
-  u32x4 ktile[kWaves][16][17];  // 272-byte rows keep the column reads conflict-free
-};
-
-// The state of row r over its keys of pages [page0, page1) of its table (keys
-// below ctx), for KV head h: G records at rec.
-template <int G>
-__device__ __forceinline__ void attend_own(unsigned char* lds_raw, const uint16_t* __restrict__ q,
-                                           const uint16_t* __restrict__ kc, const uint16_t* __restrict__ vc,
-                                           const uint32_t* __restrict__ trow, uint32_t r, uint32_t ctx, uint32_t page0,
-                                           uint32_t page1, uint32_t h, uint32_t qh, uint32_t kvh, uint32_t pages,
-                                           float* rec, uint32_t* err) {
-  constexpr uint32_t kWavePages = kOwnPages / kWaves;
-  auto& lds = *reinterpret_cast<OwnLds<G>*>(lds_raw);
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t g16 = lane >> 4, r16 = lane & 15;
-  const float kNegInf = -__builtin_inff();
-  const float cs = kScoreScale * kLog2e;
-  float* sw = &lds.sbuf[wave][0][0];
-  bool bad = false;
-  uint32_t bad_page = 0;
-
-  // B operand: query head h G + r16 (zero for r16 >= G), dims 32 i + 8 g16 .. + 7.
-  u32x4 qv[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    qv[i] = r16 < G ? *reinterpret_cast<const u32x4*>(q + ((uint64_t)r * qh + h * G + r16) * 128 + 32 * i + 8 * g16)
-                    : u32x4{0u, 0u, 0u, 0u};
-  float m[G], l[G], acc[G][2];
-#pragma unroll
-  for (int g = 0; g < G; ++g) {
-    m[g] = kNegInf;
-    l[g] = acc[g][0] = acc[g][1] = 0.f;
-  }
-  for (uint32_t at = page0; at < page1; at += kOwnPages) {
-    const uint32_t w0 = at + wave * kWavePages, np = w0 < page1 ? min(page1 - w0, kWavePages) : 0u;
-    if (np == 0) break;  // this wave has no more pages (no barrier in the loop)
-    uint32_t phys = lane < (int)np ? trow[w0 + lane] : 0u;
-    if (phys >= pages) {
-      bad_page = 1;
-      phys = 0;
-    }
-    auto phys_of = [&](uint32_t j) { return (uint32_t)__builtin_amdgcn_readlane((int)phys, (int)j); };
-    // Whole 256-byte token rows per load (lane: token 4 i + g16, dims 8 r16 .. + 7).
-    u32x4 kr[kWavePages][4];
-#pragma unroll
-    for (uint32_t u = 0; u < kWavePages; ++u)
-      if (u < np) {
-        const uint16_t* kp = kc + (((uint64_t)phys_of(u) * 16 + g16) * kvh + h) * 128 + 8 * r16;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) kr[u][i] = *reinterpret_cast<const u32x4*>(kp + (uint64_t)4 * i * kvh * 128);
-      }
-    uint32_t vd[kWavePages][16];
-#pragma unroll
-    for (uint32_t u = 0; u < kWavePages; ++u)
-      if (u < np) {
-        const uint32_t* vp = reinterpret_cast<const uint32_t*>(vc + (((uint64_t)phys_of(u) * 16) * kvh + h) * 128) + lane;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) vd[u][e] = vp[(uint64_t)e * kvh * 64];
-      }
-    // Scores: S^T = K Q^T a page at a time; lane: query r16, tokens 4 g16 + e.
-    float pm = kNegInf;
-#pragma unroll
-    for (uint32_t u = 0; u < kWavePages; ++u)
-      if (u < np) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) lds.ktile[wave][4 * i + g16][r16] = kr[u][i];
-        wave_fence();
-        f32x4 sacc = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          sacc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, lds.ktile[wave][r16][g16 + 4 * i]),
-                                                        __builtin_bit_cast(bf16x8, qv[i]), sacc, 0, 0, 0);
-        wave_fence();
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const bool valid = (w0 + u) * 16 + 4 * g16 + e < ctx;
-          const float sv = valid ? sacc[e] * cs : kNegInf;
-          bad |= valid && !is_finite_f32(sv);
-          pm = fmaxf(pm, sv);
-          if (r16 < G) sw[(u * 16 + 4 * g16 + e) * G + r16] = sv;
-        }
-      }
-    pm = fmaxf(pm, __shfl_xor(pm, 16, 64));
-    pm = fmaxf(pm, __shfl_xor(pm, 32, 64));
-    float scale[G];
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-      const float m_new = fmaxf(m[g], lane_bcast(pm, g));  // finite: a wave's pages hold a key
-      scale[g] = __builtin_amdgcn_exp2f(m[g] - m_new);
-      m[g] = m_new;
-    }
-    wave_fence();
-    // Probabilities in place, one token a lane; their sums.
-    if (lane < (int)(np * 16)) {
-#pragma unroll
-      for (int g = 0; g < G; ++g) sw[lane * G + g] = __builtin_amdgcn_exp2f(sw[lane * G + g] - m[g]);
-    }
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-      const float ps = lane < (int)(np * 16) ? sw[lane * G + g] : 0.f;
-      l[g] = l[g] * scale[g] + wave_sum(ps);
-      acc[g][0] *= scale[g];
-      acc[g][1] *= scale[g];
-    }
-    wave_fence();
-    // n += p v: lane owns dims 2 lane, 2 lane + 1.
-#pragma unroll
-    for (uint32_t u = 0; u < kWavePages; ++u)
-      if (u < np) {
-        const uint32_t valid = min(16u, ctx - (w0 + u) * 16);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const uint32_t v = (uint32_t)e < valid ? vd[u][e] : 0u;  // slots past the context may hold anything
-          const float v0 = lo_bf16(v), v1 = hi_bf16(v);
-#pragma unroll
-          for (int g = 0; g < G; ++g) {
-            const float p = sw[(u * 16 + e) * G + g];
-            acc[g][0] = __builtin_fmaf(p, v0, acc[g][0]);
-            acc[g][1] = __builtin_fmaf(p, v1, acc[g][1]);
-          }
-        }
-      }
-    wave_fence();
-  }
-  // The waves' states in wave order (a wave without pages has l = 0).
-#pragma unroll
-  for (int g = 0; g < G; ++g) {
-    if (lane == 0) {
-      lds.stat[wave][0][g] = m[g];
-      lds.stat[wave][1][g] = l[g];
-    }
-    lds.acc[wave][g][2 * lane] = acc[g][0];
-    lds.acc[wave][g][2 * lane + 1] = acc[g][1];
-  }
-  __syncthreads();
-  for (int idx = threadIdx.x; idx < G * 128; idx += kThreads) {
-    const int g = idx >> 7, c = idx & 127;
-    float M = lds.stat[0][0][g];
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) M = fmaxf(M, lds.stat[w][0][g]);
-    float n = 0.f, L = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const float lw = lds.stat[w][1][g];
-      if (lw > 0.f) {
-        const float f = __builtin_amdgcn_exp2f(lds.stat[w][0][g] - M);
-        n += lds.acc[w][g][c] * f;
-        L += lw * f;
-      }
-    }
-    rec[g * kRecord + 4 + c] = n;
-    if (c == 0) {
-      rec[g * kRecord] = M;
-      rec[g * kRecord + 1] = L;
-      bad |= !(L > 0.f);
-    }
-  }
-  if (bad) raise_error(err, ERR_NONFINITE);
-  if (bad_page) raise_error(err, ERR_PAGE);
 }
 
 // Pages of row r's own keys; 0 where the row is not computed.
@@ -486,18 +482,19 @@ __device__ __forceinline__ uint32_t own_pages(const uint32_t* positions, const G
 }
 
 // Workgroups [0, prefix_wgs): one chunk of a prefix for a block of rows and a
-// KV head. The others share the rows' own keys, cut into units of unit_pages
-// pages (a rule on the positions' total): every workgroup counts them for
-// itself, takes units own, own + own_wgs, ... of each KV head, and the first
-// one writes each row's first unit to `first` for the merge.
-template <int G, int WQ, int WK>
-__global__ __launch_bounds__(kThreads, 2) void prefix_kernel(
-    const uint16_t* __restrict__ q, const uint16_t* __restrict__ kc, const uint16_t* __restrict__ vc,
-    const uint32_t* __restrict__ positions, const uint32_t* __restrict__ table, uint32_t rows, uint32_t qh, uint32_t kvh,
-    uint32_t stride, uint32_t pages, uint32_t context, uint32_t prefix_wgs, uint32_t own_wgs, float* prefix_rec,
-    float* own_rec, uint32_t* first, uint32_t* err, Groups gs) {
+// KV head (FORM: 0 narrow, 1 and 2 the wide form's WK). The others share the
+// rows' own keys, cut into units of a number of pages that is a rule on the
+// positions' total: every workgroup counts them for itself, takes units own, own
+// + own_wgs, ... of each KV head, and the first one writes each row's first unit
+// to `first` for the merge.
+template <int G, int FORM>
+__global__ __launch_bounds__(kThreads, 4) void prefix_kernel(Args a, const uint32_t* __restrict__ positions,
+                                                             const uint32_t* __restrict__ table, uint32_t rows,
+                                                             uint32_t stride, uint32_t context, uint32_t prefix_wgs,
+                                                             uint32_t own_wgs, float* prefix_rec, float* own_rec,
+                                                             uint32_t* first, Groups gs) {
   __shared__ __attribute__((aligned(16))) unsigned char lds_raw[2 * kTileBytes];
-  static_assert(sizeof(OwnLds<G>) <= sizeof(lds_raw), "the own keys' part fits the tiles'");
+  const uint32_t kvh = a.kvh;
   if (blockIdx.x < prefix_wgs) {
     const uint32_t h = blockIdx.x % kvh, item = blockIdx.x / kvh;
     uint32_t gi = 0;
@@ -515,16 +512,22 @@ __global__ __launch_bounds__(kThreads, 2) void prefix_kernel(
       bool differ = false;
       for (uint32_t i = threadIdx.x; i < nrows * np; i += kThreads)
         differ |= table[(uint64_t)(row0 + i / np) * stride + p0 + i % np] != lead[p0 + i % np];
-      if (differ) raise_error(err, ERR_PAGE);
+      if (differ) raise_error(a.err, ERR_PAGE);
     }
-    attend_prefix<G, WQ, WK>(lds_raw, q, kc, vc, table + (uint64_t)row0 * stride, row0, nrows, key0, key1, h, qh, kvh,
-                             pages, prefix_rec, gs.prefix_slots, chunk, err);
+    const uint32_t* trow = table + (uint64_t)row0 * stride;
+    float* rec = prefix_rec + (((uint64_t)row0 * a.qh + h * G) * gs.prefix_slots + chunk) * kRecord;
+    if constexpr (FORM == 0)
+      attend_narrow<G>(lds_raw, a, trow, row0, nrows, key0, key1, h, rec, (uint64_t)a.qh * gs.prefix_slots * kRecord,
+                       (uint64_t)gs.prefix_slots * kRecord);
+    else
+      attend_wide<G, FORM>(lds_raw, a, trow, row0, nrows, key0, key1, h, rec, gs.prefix_slots);
     return;
   }
   const uint32_t own = blockIdx.x - prefix_wgs;
   __shared__ uint32_t scan[kThreads];
-  __shared__ uint32_t wave_total[kWaves];
+  __shared__ uint32_t wave_total[2][kWaves];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t turn = 0;
   // Sum over the workgroup (every thread gets it) and the sum up to this thread.
   auto block_scan = [&](uint32_t v, uint32_t& total) {
     uint32_t sum = v;
@@ -533,33 +536,40 @@ __global__ __launch_bounds__(kThreads, 2) void prefix_kernel(
       const uint32_t up = __shfl_up(sum, off, 64);
       if (lane >= off) sum += up;
     }
-    __syncthreads();
-    if (lane == 63) wave_total[wave] = sum;
+    uint32_t* t = wave_total[turn ^= 1];  // the other one may still be read
+    if (lane == 63) t[wave] = sum;
     __syncthreads();
     total = 0;
+#pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-      if (w < wave) sum += wave_total[w];
-      total += wave_total[w];
+      const uint32_t x = t[w];
+      if (w < wave) sum += x;
+      total += x;
     }
+    total = uniform(total);
     return sum;
   };
   uint64_t all = 0;
   bool bad = false;
+  uint32_t pages0 = 0;  // of this thread's row below kThreads
   for (uint32_t r0 = 0; r0 < rows; r0 += kThreads) {
     const uint32_t r = r0 + threadIdx.x;
+    const uint32_t n = r < rows ? own_pages(positions, gs, r, context, stride, bad) : 0u;
+    if (r0 == 0) pages0 = n;
     uint32_t total;
-    block_scan(r < rows ? own_pages(positions, gs, r, context, stride, bad) : 0u, total);
+    block_scan(n, total);
     all += total;
   }
-  if (bad && own == 0) raise_error(err, ERR_POSITION);
+  if (bad && own == 0) raise_error(a.err, ERR_POSITION);
   // (The cap is beyond any row: one unit each.)
-  const uint32_t unit_pages =
-      (uint32_t)min((all * kvh / kOwnUnits + kOwnPages) / kOwnPages * kOwnPages, (uint64_t)1 << 24);
-  uint32_t base = 0;  // units of the rows before r0
+  constexpr uint32_t kStepPages = kStep / 16;
+  const uint32_t unit_pages = (uint32_t)min((all * kvh / kOwnUnits + kStepPages) / kStepPages * kStepPages, (uint64_t)1 << 24);
+  uint32_t base = 0;    // units of the rows before r0
   uint32_t next = own;  // this workgroup's next (unit, head)
   for (uint32_t r0 = 0; r0 < rows; r0 += kThreads) {
     const uint32_t r = r0 + threadIdx.x;
-    const uint32_t mine = r < rows ? (own_pages(positions, gs, r, context, stride, bad) + unit_pages - 1) / unit_pages : 0u;
+    const uint32_t n = r0 == 0 ? pages0 : r < rows ? own_pages(positions, gs, r, context, stride, bad) : 0u;
+    const uint32_t mine = (n + unit_pages - 1) / unit_pages;
     uint32_t total;
     const uint32_t upto = block_scan(mine, total);
     scan[threadIdx.x] = upto;
@@ -578,13 +588,11 @@ __global__ __launch_bounds__(kThreads, 2) void prefix_kernel(
         else
           lo = mid + 1;
       }
-      const uint32_t row = __builtin_amdgcn_readfirstlane(r0 + lo);
-      const uint32_t before = lo ? scan[lo - 1] : 0u;
-      const uint32_t prefix = prefix_of(gs, row), ctx = __builtin_amdgcn_readfirstlane(positions[row]) + 1;
-      const uint32_t page0 = __builtin_amdgcn_readfirstlane(prefix / 16 + (unit - before) * unit_pages);
-      const uint32_t page1 = min(page0 + unit_pages, (ctx + 15) / 16);
-      attend_own<G>(lds_raw, q, kc, vc, table + (uint64_t)row * stride, row, ctx, page0, page1, h, qh, kvh, pages,
-                    own_rec + (uint64_t)next * G * kRecord, err);
+      const uint32_t row = uniform(r0 + lo), before = lo ? scan[lo - 1] : 0u;
+      const uint32_t prefix = prefix_of(gs, row), end = uniform(positions[row]) + 1;
+      const uint32_t key0 = uniform(prefix + (unit - before) * unit_pages * 16), key1 = min(key0 + unit_pages * 16, end);
+      attend_narrow<G>(lds_raw, a, table + (uint64_t)row * stride, row, 1, key0, key1, h,
+                       own_rec + (uint64_t)next * G * kRecord, 0, kRecord);
       __syncthreads();
     }
     base += total;
@@ -665,8 +673,8 @@ PrefixPlan prefix_plan(const fh_prefix_group* groups, uint32_t ngroups, uint32_t
     if (to.rows > most) most = to.rows;
   }
   const uint64_t vectors = (uint64_t)most * g;
-  p.form = vectors > 64 ? 1 : vectors > 32 ? 2 : 4;
-  p.gs.block_rows = 128 / p.form / g;
+  p.form = vectors > 64 ? 1 : vectors > 16 ? 2 : 0;
+  p.gs.block_rows = (p.form == 1 ? 128 : p.form == 2 ? 64 : 16) / g;
   // Two workgroups per CU over the prefixes, of at least kMinChunk tokens.
   uint64_t tokens = 0;
   for (uint32_t i = 0; i < p.gs.count; ++i)
@@ -681,7 +689,7 @@ PrefixPlan prefix_plan(const fh_prefix_group* groups, uint32_t ngroups, uint32_t
     p.items += chunks * ((to.rows + p.gs.block_rows - 1) / p.gs.block_rows);
     if (chunks > p.gs.prefix_slots) p.gs.prefix_slots = chunks;
   }
-  p.own_wgs = (uint64_t)rows * kvh < 256 ? 256 : 512;
+  p.own_wgs = kOwnWgs;
   p.prefix_floats = (uint64_t)rows * qh * p.gs.prefix_slots * kRecord;
   // Units: a row's last one may be short, the others hold at least all / kOwnUnits pages and heads.
   p.own_floats = ((uint64_t)kOwnUnits + kvh + (uint64_t)rows * kvh) * g * kRecord;
@@ -705,18 +713,18 @@ hipError_t launch_prefix_attention(const uint16_t* q, const uint16_t* k_cache, c
   float* own_rec = prefix_rec + p.prefix_floats;
   uint32_t* first = reinterpret_cast<uint32_t*>(own_rec + p.own_floats);
   const uint32_t prefix_wgs = p.items * kvh;
-#define FH_PREFIX_FORM(G_, WQ_, WK_)                                                                               \
-  hipLaunchKernelGGL((prefix_kernel<G_, WQ_, WK_>), dim3(prefix_wgs + p.own_wgs), dim3(kThreads), 0, s, q, k_cache, \
-                     v_cache, positions, table, rows, qh, kvh, stride, pages, context, prefix_wgs, p.own_wgs,      \
-                     prefix_rec, own_rec, first, err, p.gs)
-#define FH_PREFIX(G_)              \
-  do {                             \
-    if (p.form == 1)               \
-      FH_PREFIX_FORM(G_, 4, 1);    \
-    else if (p.form == 2)          \
-      FH_PREFIX_FORM(G_, 2, 2);    \
-    else                           \
-      FH_PREFIX_FORM(G_, 1, 2);    \
+  const Args a{q, k_cache, v_cache, qh, kvh, pages, err};
+#define FH_PREFIX_FORM(G_, FORM_)                                                                                 \
+  hipLaunchKernelGGL((prefix_kernel<G_, FORM_>), dim3(prefix_wgs + p.own_wgs), dim3(kThreads), 0, s, a, positions, \
+                     table, rows, stride, context, prefix_wgs, p.own_wgs, prefix_rec, own_rec, first, p.gs)
+#define FH_PREFIX(G_)            \
+  do {                           \
+    if (p.form == 1)             \
+      FH_PREFIX_FORM(G_, 1);     \
+    else if (p.form == 2)        \
+      FH_PREFIX_FORM(G_, 2);     \
+    else                         \
+      FH_PREFIX_FORM(G_, 0);     \
   } while (0)
   switch (qh / kvh) {
     case 1: FH_PREFIX(1); break;

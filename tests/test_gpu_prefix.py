@@ -183,6 +183,22 @@ def test_no_groups_is_ordinary_attention():
     holds(b, bits)
 
 
+def test_long_units_and_long_chunks():
+    """Sizes at which one workgroup walks more pages than it holds table entries for at once: 40 rows over the same
+    8300 keys without a group (own keys of 33 steps), and 1024 rows of a group (prefix chunks of 17 tiles)."""
+    b = Batch(20, [([8300], 0)], 32, 8)
+    b.table, b.lengths, b.rows = np.repeat(b.table, 40, 0), np.repeat(b.lengths, 40), 40
+    b.lengths[1::2] -= 1 + np.arange(20)
+    b.q = torch.randn(40, 32, 128, generator=torch.Generator().manual_seed(1)).bfloat16()
+    bits, err = b.device().run()
+    assert err == 0
+    holds(b, bits, [0, 1, 20, 39])
+    b = Batch(21, [([1 + i % 5 for i in range(1024)], 132)], 32, 8).device()
+    bits, err = b.run()
+    assert err == 0
+    holds(b, bits, [0, 1, 33, 500, 1023])
+
+
 def test_groups_change_the_order_of_sums_only():
     """The same rows with their shared prefix given whole, in part, and not at all."""
     b = Batch(4, [([40, 3, 77, 1, 250], 30)], 32, 8).device()
