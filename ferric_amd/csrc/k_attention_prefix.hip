@@ -55,8 +55,10 @@ constexpr int kKeys = 64;             // keys per tile of the wide form
 constexpr int kStep = 32 * kWaves;    // keys of the narrow form's waves at once
 constexpr size_t kTileBytes = 16 * 2 * kKeys * 16;  // K or V, double-buffered
 constexpr uint32_t kMinChunk = 256;   // least tokens of a prefix chunk
-constexpr uint32_t kOwnUnits = 256;   // own keys are cut into about this many units
-constexpr uint32_t kOwnWgs = 256;     // workgroups that take them
+constexpr uint32_t kPartKeys = 512;   // least own keys of a part where a row has several
+constexpr uint32_t kMaxParts = 32;
+constexpr uint32_t kSlots = 512;      // workgroups that run at once: two on each CU
+constexpr uint32_t kVectors = 16;     // of a wave
 // f32(0x3db504f3) (1/sqrt(128), paged_decode.rs:31-35) times log2 e.
 constexpr float kScoreScale = 0.08838834764831845f * 1.44269504088896341f;
 constexpr uint32_t kRecord = 132;     // m, l, two unused, n[128]: 16-byte aligned
@@ -116,8 +118,7 @@ struct State {
     for (int d = 0; d < 8; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  // Takes in T tiles of 16 scores: keys first + 16 t + 4 (lane / 16) + e below `end`. v_at(t, d): the V^T
-  // operand of tiles t, t + 1 (t even) for dims 16 d .. + 15.
+  // Takes in T tiles of 16 scores: keys first + 16 t + 4 (lane / 16) + e below `end`. v_at(t, d, v): the V^T operands of tiles t, t + 1 (t even) for dims 16 d .. + 63.
   template <int T, class V>
   __device__ __forceinline__ void take(f32x4 (&s)[T], uint32_t first, uint32_t end, const V& v_at) {
     const float kNegInf = -__builtin_inff();
@@ -156,6 +157,10 @@ struct State {
         for (int e = 0; e < 4; ++e) acc[d][e] *= a;
     }
     const float mc = m == kNegInf ? 0.f : m * kScoreScale;
+    // 32 keys at a time; the V operands of four dim tiles are requested before the MFMAs of the four before them,
+    // the first ones before the exponentials.
+    bf16x8 va[2][4];
+    v_at(0, 0, va[0]);
 #pragma unroll
     for (int t = 0; t < T; t += 2) {
       float p[8];
@@ -168,15 +173,25 @@ struct State {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         ph[e] = pack_bf16x2(p[2 * e], p[2 * e + 1]);
+        asm volatile("" : "+v"(ph[e]));  // its halves by shift and mask, not by rounding again
         pl[e] = pack_bf16x2(p[2 * e] - lo_bf16(ph[e]), p[2 * e + 1] - hi_bf16(ph[e]));
       }
       const bf16x8 bh = __builtin_bit_cast(bf16x8, u32x4{ph[0], ph[1], ph[2], ph[3]});
       const bf16x8 bl = __builtin_bit_cast(bf16x8, u32x4{pl[0], pl[1], pl[2], pl[3]});
 #pragma unroll
-      for (int d = 0; d < 8; ++d) {
-        const bf16x8 va = v_at(t, d);
-        acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, bh, acc[d], 0, 0, 0);
-        acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, bl, acc[d], 0, 0, 0);
+      for (int half = 0; half < 2; ++half) {
+        if (half == 0)
+          v_at(t, 4, va[1]);
+        else if (t + 2 < T)
+          v_at(t + 2, 0, va[0]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+          acc[4 * half + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va[half][d], bh, acc[4 * half + d], 0, 0, 0);
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+          acc[4 * half + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va[half][d], bl, acc[4 * half + d], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
@@ -188,20 +203,35 @@ struct State {
   }
 };
 
-// Transposing reads of V^T from LDS rows of tokens (u32x4[16] each): keys 16 t + 4 (lane / 16) + 0..3 of
-// tiles t and t + 1, dims 16 d .. + 15.
-__device__ __forceinline__ bf16x8 v_operand(const u32x4 (*rows)[16], int t, int d) {
-  const int lane = threadIdx.x & 63;
+typedef __attribute__((address_space(3))) unsigned char* LdsBytes;
+
+// Transposing reads of V^T from LDS rows of tokens (256 bytes each): keys 16 t + 4 (lane / 16) + 0..3 of tiles t and
+// t + 1, dims 16 d .. + 63. lane_v: a lane's address part, v_lane(); the chunk permutation makes dims 16 d of it an
+// exclusive or with 32 d.
+__device__ __forceinline__ uint32_t v_lane(int lane) {
   const uint32_t j = lane & 15, key = 4 * (lane >> 4) + (j >> 2);
-  u32x2 v[2];
+  return key * 256 + 32 * (key & 7) + 8 * (j & 3);
+}
+__device__ __forceinline__ void v_operands(LdsBytes rows, uint32_t lane_v, int t, int d, bf16x8 (&v)[4]) {
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const uint32_t k = 16 * (t + u) + key, c = (2 * d + ((j & 3) >> 1)) ^ (2 * (key & 7));
-    auto* src = reinterpret_cast<u32x2*>(const_cast<u32x4*>(&rows[k][c])) + (j & 1);
-    v[u] = __builtin_bit_cast(u32x2,
-                              __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)src));
+  for (int i = 0; i < 4; ++i) {
+    u32x2 w[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      w[u] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                           (__attribute__((address_space(3))) s16x4*)(rows + (lane_v ^ (32 * (d + i))) +
+                                                                                      (t + u) * 4096)));
+    v[i] = __builtin_bit_cast(bf16x8, u32x4{w[0][0], w[0][1], w[1][0], w[1][1]});
   }
-  return __builtin_bit_cast(bf16x8, u32x4{v[0][0], v[0][1], v[1][0], v[1][1]});
+}
+// K operand of one 16-key tile: keys lane % 16, dims 32 i + 8 (lane / 16) .. + 7, i = 0..3.
+__device__ __forceinline__ uint32_t k_lane(int lane) {
+  return (lane & 15) * 256 + 16 * ((lane >> 4) ^ (lane & 15));
+}
+__device__ __forceinline__ void k_operands(LdsBytes rows, uint32_t lane_k, bf16x8 (&k)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    k[i] = *(__attribute__((address_space(3))) bf16x8*)(rows + (lane_k ^ (64 * i)));
 }
 
 // Query operand: vector lane % 16 of the wave's 16 (vector `vec` of nrows rows), dims 32 i + 8 (lane / 16) .. + 7.
@@ -244,8 +274,9 @@ __device__ __forceinline__ Page page_of(const Args& a, uint32_t page, uint32_t v
 }
 
 // The wide form: nrows rows from row0 on (sharing trow's pages), keys [key0, key1) of KV head h, key0 a
-// multiple of 16. WK waves share a tile's keys, 8 / WK own the vectors. rec: record of (row 0, head 0), row
-// and head steps of `slots` records.
+// multiple of 16. The waves share 64-key tiles, the next one in flight: 8 / WK waves own the vectors; with WK = 2 two
+// waves share them and take half of a tile's keys each. rec: record of (row 0, head 0), row and head steps of `slots`
+// records.
 template <int G, int WK>
 __device__ __forceinline__ void attend_wide(unsigned char* lds_raw, const Args& a, const uint32_t* __restrict__ trow,
                                             uint32_t row0, uint32_t nrows, uint32_t key0, uint32_t key1, uint32_t h,
@@ -259,8 +290,8 @@ __device__ __forceinline__ void attend_wide(unsigned char* lds_raw, const Args& 
   // Page-table entries of 64 pages, one per lane, the next 64 requested ahead.
   auto table_chunk = [&](uint32_t first) { return first + lane < npages ? trow[page0 + first + lane] : 0u; };
   uint32_t tab = table_chunk(0), tab_next = table_chunk(64);
-  // Waves 0..3 copy K of the tile's pages 0..3, waves 4..7 V: four tokens per load (lane: token 4 i + lane /
-  // 16, LDS chunk lane % 16).
+  // Waves 0..3 copy K of the tile's pages 0..3, waves 4..7 V: four tokens per load (lane: token 4 i + lane / 16, LDS
+  // chunk lane % 16).
   const int my_page = wave & 3;
   const bool is_v = wave >= 4;
   uint32_t off[4], bad_page = 0;
@@ -269,22 +300,23 @@ __device__ __forceinline__ void attend_wide(unsigned char* lds_raw, const Args& 
     const uint32_t token = 4 * i + (lane >> 4), swizzle = is_v ? 2 * (token & 7) : token;
     off[i] = token * a.kvh * 256 + (((lane & 15) ^ swizzle) & 15) * 16;
   }
-  auto fetch = [&](uint32_t t, int buf) {
+  auto fetch = [&](uint32_t t) {
     const uint32_t pi = 4 * t + my_page;
     const uint32_t page = (uint32_t)__builtin_amdgcn_readlane((int)tab, (int)(pi & 63u));
     const Page p = page_of(a, page, pi < npages ? min(16u, key1 - key0 - pi * 16) : 0u, h, bad_page);
     auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)((is_v ? a.vc : a.kc) + p.base), 0, p.bytes, 0x00020000);
-    u32x4(*to)[16] = is_v ? vlds[buf] : klds[buf];
+    u32x4(*to)[16] = (is_v ? vlds : klds)[t & 1];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
           rsrc, (__attribute__((address_space(3))) void*)&to[16 * my_page + 4 * i][0], 16, off[i], 0, 0, 0);
   };
-  fetch(0, 0);
-  const uint32_t vec = 16 * wq + (lane & 15);
-  const bool live = (uint32_t)(16 * wq) < nrows * G;  // a wave with no vectors only fetches
+  fetch(0);
+  const uint32_t vec = kVectors * wq + (lane & 15);
+  const bool live = (uint32_t)(kVectors * wq) < nrows * G;  // a wave with no vectors only fetches
   u32x4 qv[4];
   load_q<G>(qv, a, row0, nrows, vec, h);
+  uint32_t lane_k = k_lane(lane), lane_v = v_lane(lane);
   State st;
   st.clear();
   for (uint32_t t = 0; t < tiles; ++t) {
@@ -295,23 +327,27 @@ __device__ __forceinline__ void attend_wide(unsigned char* lds_raw, const Args& 
         tab = tab_next;
         tab_next = table_chunk(4 * (t + 1) + 64);
       }
-      fetch(t + 1, (t + 1) & 1);
+      fetch(t + 1);
     }
     if (!live) continue;
-    const int buf = t & 1, mine = kTiles * wk;
+    asm volatile("" : "+v"(lane_k), "+v"(lane_v));  // the reads' addresses are made here each time: kept, they spill
+    const int mine = kTiles * wk;
+    const LdsBytes kb = (LdsBytes)&klds[t & 1][16 * mine][0], vb = (LdsBytes)&vlds[t & 1][16 * mine][0];
     f32x4 s[kTiles];
 #pragma unroll
-    for (int u = 0; u < kTiles; ++u) {
-      s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int u = 0; u < kTiles; u += 2) {
+      bf16x8 k[2][4];
+      k_operands(kb + u * 4096, lane_k, k[0]);
+      k_operands(kb + (u + 1) * 4096, lane_k, k[1]);
+      s[u] = s[u + 1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const u32x4 ka = klds[buf][16 * (mine + u) + (lane & 15)][(4 * i + (lane >> 4)) ^ (lane & 15)];
-        s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, ka), __builtin_bit_cast(bf16x8, qv[i]),
-                                                       s[u], 0, 0, 0);
-      }
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+          s[u + w] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[w][i], __builtin_bit_cast(bf16x8, qv[i]), s[u + w], 0, 0, 0);
     }
     st.template take<kTiles>(s, key0 + t * kKeys + 16 * mine, key1,
-                             [&](int u, int d) { return v_operand(&vlds[buf][16 * mine], u, d); });
+                             [&](int u, int d, bf16x8(&v)[4]) { v_operands(vb, lane_v, u, d, v); });
   }
   st.finish();
   if constexpr (WK == 2) {
@@ -352,16 +388,18 @@ __device__ __forceinline__ void attend_wide(unsigned char* lds_raw, const Args& 
 
 // LDS of the narrow form: V of each wave's 32 keys, then the waves' states.
 struct NarrowState {
-  float acc[kWaves][16][128];
+  float acc[kWaves][kVectors][128];
 };
 static_assert(sizeof(NarrowState) == 2 * kTileBytes, "the states of 8 waves fill the tiles' LDS");
+struct NarrowSums {
+  float m[kWaves][kVectors], l[kWaves][kVectors];  // m in the exponent of 2
+};
 
-// The narrow form: as above for nrows * G <= 16 vectors. The record of vector v is rec + (v / G) * row_step +
-// (v % G) * head_step.
+// The narrow form: as above for nrows * G <= 16 vectors; the waves' states are left in LDS, behind a barrier.
 template <int G>
-__device__ __forceinline__ void attend_narrow(unsigned char* lds_raw, const Args& a, const uint32_t* __restrict__ trow,
-                                              uint32_t row0, uint32_t nrows, uint32_t key0, uint32_t key1, uint32_t h,
-                                              float* rec, uint64_t row_step, uint64_t head_step) {
+__device__ __forceinline__ void attend_narrow(unsigned char* lds_raw, NarrowSums& sums, const Args& a,
+                                              const uint32_t* __restrict__ trow, uint32_t row0, uint32_t nrows,
+                                              uint32_t key0, uint32_t key1, uint32_t h) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   u32x4(*vlds)[16] = reinterpret_cast<u32x4(*)[16]>(lds_raw) + 32 * wave;
   const uint32_t page0 = key0 / 16, npages = (key1 - key0 + 15) / 16, steps = (key1 - key0 + kStep - 1) / kStep;
@@ -380,8 +418,10 @@ __device__ __forceinline__ void attend_narrow(unsigned char* lds_raw, const Args
     const uint32_t token = 4 * i + (lane >> 4);
     voff[i] = token * a.kvh * 256 + (((lane & 15) ^ (2 * (token & 7))) & 15) * 16;
   }
+  uint32_t lane_v = v_lane(lane);
   State st;
   st.clear();
+#pragma unroll 1
   for (uint32_t step = 0; step < steps; ++step) {
     const uint32_t first = step * kStep + 32 * wave;  // key0-relative
     if (first >= key1 - key0) break;  // no more keys for this wave (no barrier in the loop)
@@ -410,58 +450,69 @@ __device__ __forceinline__ void attend_narrow(unsigned char* lds_raw, const Args
     __builtin_amdgcn_s_waitcnt(0 | (7u << 4) | (15u << 8));
     wave_fence();
     f32x4 s[2];
+    s[0] = s[1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int u = 0; u < 2; ++u)
         s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kr[u][i]),
                                                        __builtin_bit_cast(bf16x8, qv[i]), s[u], 0, 0, 0);
-    }
-    st.template take<2>(s, key0 + first, key1, [&](int u, int d) { return v_operand(vlds, u, d); });
+    asm volatile("" : "+v"(lane_v));  // V's read addresses are made here, not kept beside K
+    st.template take<2>(s, key0 + first, key1,
+                        [&](int u, int d, bf16x8(&v)[4]) { v_operands((LdsBytes)vlds, lane_v, u, d, v); });
     // The next step's loads overwrite V: this step's reads of it are done.
     __builtin_amdgcn_s_waitcnt(15u | (3u << 14) | (7u << 4) | (0u << 8));
     wave_fence();
   }
   st.finish();
-  // The waves' states meet in LDS, the waves in order (one without keys has l = 0 and m = -inf).
-  __shared__ float wm[kWaves][16], wl[kWaves][16];
   __syncthreads();  // every wave is done with its V
   auto& all = *reinterpret_cast<NarrowState*>(lds_raw);
-  const uint32_t vec = lane & 15, nvec = nrows * G;
-  if (vec < nvec) {
+  const uint32_t vec = lane & 15;
+  if (vec < nrows * G) {
 #pragma unroll
     for (int d = 0; d < 8; ++d) *reinterpret_cast<f32x4*>(&all.acc[wave][vec][16 * d + 4 * (lane >> 4)]) = st.acc[d];
     if (lane < 16) {
-      wm[wave][vec] = st.m * kScoreScale;
-      wl[wave][vec] = st.l;
+      sums.m[wave][vec] = st.m * kScoreScale;
+      sums.l[wave][vec] = st.l;
     }
     if (st.l != st.l || !(st.s_abs < __builtin_inff())) raise_error(a.err, ERR_NONFINITE);
   }
   if (bad_page != 0 && lane == 0) raise_error(a.err, ERR_PAGE);
   __syncthreads();
-  for (uint32_t idx = threadIdx.x; idx < nvec * 32; idx += kThreads) {
-    const uint32_t v = idx >> 5, c = idx & 31;  // four dims
-    float M = wm[0][v];
+}
+
+// A state over some keys: the vector's maximum (in the exponent of 2), its sum and four of its dims.
+struct Part {
+  float m, l;
+  f32x4 n;
+};
+__device__ __forceinline__ Part no_part() { return Part{-__builtin_inff(), 0.f, f32x4{0.f, 0.f, 0.f, 0.f}}; }
+// The union's state. (One without keys has m = -inf and l = 0.)
+__device__ __forceinline__ Part join(const Part& x, const Part& y) {
+  const float m = fmaxf(x.m, y.m);
+  const float fx = x.m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(x.m - m);
+  const float fy = y.m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(y.m - m);
+  Part o{m, x.l * fx + y.l * fy, f32x4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) M = fmaxf(M, wm[w][v]);
-    f32x4 n = f32x4{0.f, 0.f, 0.f, 0.f};
-    float L = 0.f;
+  for (int e = 0; e < 4; ++e) o.n[e] = x.n[e] * fx + y.n[e] * fy;
+  return o;
+}
+
+// The waves' states of vector v, dims 4 c .. 4 c + 3, joined in wave order (the maximum first, then one sum).
+__device__ __forceinline__ Part narrow_part(unsigned char* lds_raw, const NarrowSums& sums, uint32_t v, uint32_t c) {
+  auto& all = *reinterpret_cast<NarrowState*>(lds_raw);
+  Part o = no_part();
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const float f = wl[w][v] > 0.f ? __builtin_amdgcn_exp2f(wm[w][v] - M) : 0.f;
-      const f32x4 x = *reinterpret_cast<const f32x4*>(&all.acc[w][v][4 * c]);
-      L += wl[w][v] * f;
+  for (int w = 0; w < kWaves; ++w) o.m = fmaxf(o.m, sums.m[w][v]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) n[e] += x[e] * f;
-    }
-    float* r = rec + (v / G) * row_step + (v % G) * head_step;
-    *reinterpret_cast<f32x4*>(r + 4 + 4 * c) = n;
-    if (c == 0) {
-      r[0] = M;
-      r[1] = L;
-    }
+  for (int w = 0; w < kWaves; ++w) {
+    const float f = sums.m[w][v] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(sums.m[w][v] - o.m);
+    const f32x4 x = *reinterpret_cast<const f32x4*>(&all.acc[w][v][4 * c]);
+    o.l += sums.l[w][v] * f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o.n[e] += x[e] * f;
   }
+  return o;
 }
 
 __device__ __forceinline__ uint32_t prefix_of(const Groups& gs, uint32_t r) {
@@ -470,196 +521,167 @@ __device__ __forceinline__ uint32_t prefix_of(const Groups& gs, uint32_t r) {
   return 0;
 }
 
-// Pages of row r's own keys; 0 where the row is not computed.
-__device__ __forceinline__ uint32_t own_pages(const uint32_t* positions, const Groups& gs, uint32_t r, uint32_t context,
-                                              uint32_t stride, bool& bad) {
-  const uint32_t pos = positions[r], prefix = prefix_of(gs, r);
-  if (pos >= context || pos / 16 >= stride || pos + 1 < prefix) {
-    bad = true;
-    return 0;
+// First launch: a workgroup takes one chunk of a prefix for a block of rows and a KV
+// head (FORM: 0 narrow, 1 and 2 the wide form's WK); its records wait in the
+// scratch. The first workgroup clears the counters of the second launch.
+template <int G, int FORM>
+__global__ __launch_bounds__(kThreads, 4) void prefix_kernel(Args a, const uint32_t* __restrict__ table, uint32_t stride,
+                                                             uint32_t items, float* rec, uint32_t* counters,
+                                                             uint32_t ncounters, Groups gs) {
+  __shared__ __attribute__((aligned(16))) unsigned char lds_raw[2 * kTileBytes];
+  const uint32_t h = blockIdx.x % a.kvh, item = blockIdx.x / a.kvh;
+  if (blockIdx.x == 0 && threadIdx.x < ncounters) counters[threadIdx.x] = 0u;
+  if (item >= items) return;
+  uint32_t gi = 0;
+  while (gi + 1 < gs.count && item >= gs.g[gi + 1].item0) ++gi;
+  const Group g = gs.g[gi];
+  const uint32_t blocks = (g.rows + gs.block_rows - 1) / gs.block_rows;
+  const uint32_t block = (item - g.item0) % blocks, chunk = (item - g.item0) / blocks;
+  const uint32_t in = block * gs.block_rows, nrows = min(gs.block_rows, g.rows - in);
+  const uint32_t key0 = chunk * gs.chunk, key1 = min(key0 + gs.chunk, g.prefix_tokens);
+  const uint32_t row0 = g.first_row + in;
+  const uint32_t* trow = table + (uint64_t)row0 * stride;
+  rec += (((uint64_t)row0 * a.qh + h * G) * gs.prefix_slots + chunk) * kRecord;
+  if constexpr (FORM == 0) {
+    __shared__ NarrowSums sums;
+    attend_narrow<G>(lds_raw, sums, a, trow, row0, nrows, key0, key1, h);
+    for (uint32_t idx = threadIdx.x; idx < nrows * G * 32; idx += kThreads) {
+      const uint32_t v = idx >> 5, c = idx & 31;
+      const Part o = narrow_part(lds_raw, sums, v, c);
+      float* r = rec + ((uint64_t)(v / G) * a.qh + v % G) * gs.prefix_slots * kRecord;
+      *reinterpret_cast<f32x4*>(r + 4 + 4 * c) = o.n;
+      if (c == 0) *reinterpret_cast<float2*>(r) = make_float2(o.m, o.l);
+    }
+  } else {
+    attend_wide<G, FORM>(lds_raw, a, trow, row0, nrows, key0, key1, h, rec, gs.prefix_slots);
   }
-  return (pos + 1 - prefix + 15) / 16;
+  if (h == 0) {
+    // The rows of the block list the same pages here as the group's first row.
+    const uint32_t p0 = key0 / 16, np = (key1 - key0 + 15) / 16;
+    const uint32_t* lead = table + (uint64_t)g.first_row * stride;
+    bool differ = false;
+    for (uint32_t i = threadIdx.x; i < nrows * np; i += kThreads)
+      differ |= table[(uint64_t)(row0 + i / np) * stride + p0 + i % np] != lead[p0 + i % np];
+    if (differ) raise_error(a.err, ERR_PAGE);
+  }
 }
 
-// Workgroups [0, prefix_wgs): one chunk of a prefix for a block of rows and a
-// KV head (FORM: 0 narrow, 1 and 2 the wide form's WK). The others share the
-// rows' own keys, cut into units of a number of pages that is a rule on the
-// positions' total: every workgroup counts them for itself, takes units own, own
-// + own_wgs, ... of each KV head, and the first one writes each row's first unit
-// to `first` for the merge.
-template <int G, int FORM>
-__global__ __launch_bounds__(kThreads, 4) void prefix_kernel(Args a, const uint32_t* __restrict__ positions,
-                                                             const uint32_t* __restrict__ table, uint32_t rows,
-                                                             uint32_t stride, uint32_t context, uint32_t prefix_wgs,
-                                                             uint32_t own_wgs, float* prefix_rec, float* own_rec,
-                                                             uint32_t* first, Groups gs) {
+// Second launch: (KV head, row, part) takes a part of the row's own keys, which are
+// cut into at most `parts` equal ones of at least kPartKeys keys, and the first part
+// the records of the prefix's chunks too. A row of one part ends here; the parts
+// of longer ones leave records, and the last one to arrive (a counter per row and KV
+// head, which the first launch cleared) joins them in key order. Records and counter
+// go through agent-scope atomics: the XCDs' L2 caches are not coherent with one
+// another. As in k_attention.hip this rests on gfx950's lowering of them (stores
+// written through, a wait that covers their completion, loads that bypass the L2).
+#if defined(__HIP_DEVICE_COMPILE__) && !defined(__gfx950__)
+#error "k_attention_prefix.hip: the in-kernel merge is written for gfx950's memory-model lowering"
+#endif
+template <int G>
+__global__ __launch_bounds__(kThreads, 4) void own_kernel(Args a, const uint32_t* __restrict__ positions,
+                                                          const uint32_t* __restrict__ table, uint32_t rows,
+                                                          uint32_t stride, uint32_t context, uint32_t max_parts,
+                                                          const float* __restrict__ prefix_rec, float* part_rec,
+                                                          uint32_t* counters, uint16_t* __restrict__ out,
+                                                          uint32_t out_mtiles, Groups gs) {
+  constexpr uint32_t kDims = G * 32;                // (vector, four dims) pairs
+  constexpr uint32_t kTeams = kThreads / kDims;     // threads per pair, for the prefix's records
+  constexpr int kInFlight = 4;
   __shared__ __attribute__((aligned(16))) unsigned char lds_raw[2 * kTileBytes];
-  const uint32_t kvh = a.kvh;
-  if (blockIdx.x < prefix_wgs) {
-    const uint32_t h = blockIdx.x % kvh, item = blockIdx.x / kvh;
-    uint32_t gi = 0;
-    while (gi + 1 < gs.count && item >= gs.g[gi + 1].item0) ++gi;
-    const Group g = gs.g[gi];
-    const uint32_t blocks = (g.rows + gs.block_rows - 1) / gs.block_rows;
-    const uint32_t block = (item - g.item0) % blocks, chunk = (item - g.item0) / blocks;
-    const uint32_t in = block * gs.block_rows, nrows = min(gs.block_rows, g.rows - in);
-    const uint32_t key0 = chunk * gs.chunk, key1 = min(key0 + gs.chunk, g.prefix_tokens);
-    const uint32_t row0 = g.first_row + in;
-    if (h == 0) {
-      // The rows of the block list the same pages here as the group's first row.
-      const uint32_t p0 = key0 / 16, np = (key1 - key0 + 15) / 16;
-      const uint32_t* lead = table + (uint64_t)g.first_row * stride;
-      bool differ = false;
-      for (uint32_t i = threadIdx.x; i < nrows * np; i += kThreads)
-        differ |= table[(uint64_t)(row0 + i / np) * stride + p0 + i % np] != lead[p0 + i % np];
-      if (differ) raise_error(a.err, ERR_PAGE);
-    }
-    const uint32_t* trow = table + (uint64_t)row0 * stride;
-    float* rec = prefix_rec + (((uint64_t)row0 * a.qh + h * G) * gs.prefix_slots + chunk) * kRecord;
-    if constexpr (FORM == 0)
-      attend_narrow<G>(lds_raw, a, trow, row0, nrows, key0, key1, h, rec, (uint64_t)a.qh * gs.prefix_slots * kRecord,
-                       (uint64_t)gs.prefix_slots * kRecord);
-    else
-      attend_wide<G, FORM>(lds_raw, a, trow, row0, nrows, key0, key1, h, rec, gs.prefix_slots);
+  __shared__ NarrowSums sums;
+  __shared__ f32x4 team_n[kTeams][kDims];
+  __shared__ float team_m[kTeams][G], team_l[kTeams][G];
+  const uint32_t h = blockIdx.x % a.kvh, r = blockIdx.x / a.kvh % rows, part = blockIdx.x / a.kvh / rows;
+  const uint32_t pos = uniform(positions[r]), prefix = prefix_of(gs, r);
+  if (pos >= context || pos / 16 >= stride || pos + 1 < prefix) {
+    if (part == 0 && h == 0 && threadIdx.x == 0) raise_error(a.err, ERR_POSITION);
     return;
   }
-  const uint32_t own = blockIdx.x - prefix_wgs;
-  __shared__ uint32_t scan[kThreads];
-  __shared__ uint32_t wave_total[2][kWaves];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  uint32_t turn = 0;
-  // Sum over the workgroup (every thread gets it) and the sum up to this thread.
-  auto block_scan = [&](uint32_t v, uint32_t& total) {
-    uint32_t sum = v;
+  const uint32_t own = pos + 1 - prefix;
+  const uint32_t wanted = max(1u, min(max_parts, own / kPartKeys));
+  const uint32_t keys = (own + wanted * kStep - 1) / (wanted * kStep) * kStep;  // of a part
+  const uint32_t parts = own > keys ? (own + keys - 1) / keys : 1u;
+  if (part >= parts) return;
+  const uint32_t v = threadIdx.x % kDims / 32, c = threadIdx.x % 32, team = threadIdx.x / kDims;
+  if (part == 0) {
+    // The prefix's chunks, every kTeams-th one, kInFlight records at a time.
+    Part t = no_part();
+    const uint32_t chunks = (prefix + gs.chunk - 1) / gs.chunk;
+    const float* p = prefix_rec + ((uint64_t)r * a.qh + h * G + v) * gs.prefix_slots * kRecord;
+    for (uint32_t i0 = team; i0 < chunks; i0 += kTeams * kInFlight) {
+      Part x[kInFlight];
 #pragma unroll
-    for (int off = 1; off < 64; off *= 2) {
-      const uint32_t up = __shfl_up(sum, off, 64);
-      if (lane >= off) sum += up;
-    }
-    uint32_t* t = wave_total[turn ^= 1];  // the other one may still be read
-    if (lane == 63) t[wave] = sum;
-    __syncthreads();
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const uint32_t x = t[w];
-      if (w < wave) sum += x;
-      total += x;
-    }
-    total = uniform(total);
-    return sum;
-  };
-  uint64_t all = 0;
-  bool bad = false;
-  uint32_t pages0 = 0;  // of this thread's row below kThreads
-  for (uint32_t r0 = 0; r0 < rows; r0 += kThreads) {
-    const uint32_t r = r0 + threadIdx.x;
-    const uint32_t n = r < rows ? own_pages(positions, gs, r, context, stride, bad) : 0u;
-    if (r0 == 0) pages0 = n;
-    uint32_t total;
-    block_scan(n, total);
-    all += total;
-  }
-  if (bad && own == 0) raise_error(a.err, ERR_POSITION);
-  // (The cap is beyond any row: one unit each.)
-  constexpr uint32_t kStepPages = kStep / 16;
-  const uint32_t unit_pages = (uint32_t)min((all * kvh / kOwnUnits + kStepPages) / kStepPages * kStepPages, (uint64_t)1 << 24);
-  uint32_t base = 0;    // units of the rows before r0
-  uint32_t next = own;  // this workgroup's next (unit, head)
-  for (uint32_t r0 = 0; r0 < rows; r0 += kThreads) {
-    const uint32_t r = r0 + threadIdx.x;
-    const uint32_t n = r0 == 0 ? pages0 : r < rows ? own_pages(positions, gs, r, context, stride, bad) : 0u;
-    const uint32_t mine = (n + unit_pages - 1) / unit_pages;
-    uint32_t total;
-    const uint32_t upto = block_scan(mine, total);
-    scan[threadIdx.x] = upto;
-    if (own == 0 && r < rows) {
-      first[r] = base + upto - mine;
-      if (r == rows - 1) first[rows] = base + upto;
-    }
-    __syncthreads();
-    for (; next < (base + total) * kvh; next += own_wgs) {
-      const uint32_t unit = next / kvh - base, h = next % kvh;
-      uint32_t lo = 0, hi = kThreads - 1;  // the first row whose units end after this one
-      while (lo < hi) {
-        const uint32_t mid = (lo + hi) / 2;
-        if (scan[mid] > unit)
-          hi = mid;
-        else
-          lo = mid + 1;
+      for (int u = 0; u < kInFlight; ++u) {
+        const float* s = p + (uint64_t)min(i0 + u * kTeams, chunks - 1) * kRecord;
+        const float2 ml = *reinterpret_cast<const float2*>(s);
+        x[u] = Part{ml.x, ml.y, *reinterpret_cast<const f32x4*>(s + 4 + 4 * c)};
       }
-      const uint32_t row = uniform(r0 + lo), before = lo ? scan[lo - 1] : 0u;
-      const uint32_t prefix = prefix_of(gs, row), end = uniform(positions[row]) + 1;
-      const uint32_t key0 = uniform(prefix + (unit - before) * unit_pages * 16), key1 = min(key0 + unit_pages * 16, end);
-      attend_narrow<G>(lds_raw, a, table + (uint64_t)row * stride, row, 1, key0, key1, h,
-                       own_rec + (uint64_t)next * G * kRecord, 0, kRecord);
-      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < kInFlight; ++u)
+        if (i0 + u * kTeams < chunks) t = join(t, x[u]);
     }
-    base += total;
-    __syncthreads();
+    team_n[team][threadIdx.x % kDims] = t.n;
+    if (c == 0) {
+      team_m[team][v] = t.m;
+      team_l[team][v] = t.l;
+    }
   }
+  const uint32_t key0 = prefix + part * keys, key1 = min(key0 + keys, pos + 1);
+  attend_narrow<G>(lds_raw, sums, a, table + (uint64_t)r * stride, r, 1, key0, key1, h);
+  const bool mine = threadIdx.x < kDims;
+  Part o = no_part();
+  if (mine) {
+    if (part == 0)
+#pragma unroll
+      for (uint32_t t = 0; t < kTeams; ++t) o = join(o, Part{team_m[t][v], team_l[t][v], team_n[t][threadIdx.x]});
+    o = join(o, narrow_part(lds_raw, sums, v, c));
+  }
+  if (parts > 1) {
+    __shared__ uint32_t last;
+    float* to = part_rec + (((uint64_t)r * a.kvh + h) * max_parts * G + v) * kRecord;
+    if (mine) {
+      float* x = to + (uint64_t)part * G * kRecord;
+      if (c == 0) {
+        __hip_atomic_store(x, o.m, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(x + 1, o.l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        __hip_atomic_store(x + 4 + 4 * c + e, o.n[e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (threadIdx.x == 0) last = atomicAdd(counters + (uint64_t)r * a.kvh + h, 1u) == parts - 1 ? 1u : 0u;
+    __syncthreads();
+    if (!last) return;
+    if (mine) {
+      o = no_part();
+      for (uint32_t i = 0; i < parts; ++i) {
+        const float* x = to + (uint64_t)i * G * kRecord;
+        Part y;
+        y.m = __hip_atomic_load(x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        y.l = __hip_atomic_load(x + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y.n[e] = __hip_atomic_load(x + 4 + 4 * c + e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        o = join(o, y);
+      }
+    }
+  }
+  if (!mine) return;
+  const uint32_t w0 = pack_bf16x2(o.n[0] / o.l, o.n[1] / o.l), w1 = pack_bf16x2(o.n[2] / o.l, o.n[3] / o.l);
+  const uint32_t col = (h * G + v) * 128 + 4 * c;
+  uint16_t* dst = out_mtiles ? out + act_offset_m(r, col, out_mtiles) : out + (uint64_t)r * a.qh * 128 + col;
+  *reinterpret_cast<uint2*>(dst) = make_uint2(w0, w1);
+  auto inf = [](uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; };
+  if (!(o.l > 0.f) || inf(w0) || inf(w1)) raise_error(a.err, ERR_NONFINITE);
 }
 
-// One wave per (row, query head): its records in ascending key order, the
-// prefix's chunks and then its own units. Up to 64 records at a time: lane i
-// holds record i's weight, then every lane its two dims of eight records at once.
-__global__ __launch_bounds__(256) void prefix_merge_kernel(const float* __restrict__ prefix_rec,
-                                                          const float* __restrict__ own_rec,
-                                                          const uint32_t* __restrict__ first,
-                                                          const uint32_t* __restrict__ positions,
-                                                          uint16_t* __restrict__ out, uint32_t out_mtiles, uint32_t rows,
-                                                          uint32_t qh, uint32_t kvh, uint32_t stride, uint32_t context,
-                                                          uint32_t* err, Groups gs) {
-  const int lane = threadIdx.x & 63;
-  const uint32_t id = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = id / qh, head = id % qh;
-  if (r >= rows) return;
-  const uint32_t pos = positions[r], prefix = prefix_of(gs, r);
-  if (pos >= context || pos / 16 >= stride || pos + 1 < prefix) return;  // reported by the own keys' part
-  const uint32_t u0 = first[r], np = (prefix + gs.chunk - 1) / gs.chunk, n = np + first[r + 1] - u0;
-  const uint32_t g = qh / kvh;
-  const float* pp = prefix_rec + (uint64_t)id * gs.prefix_slots * kRecord;
-  const float* po = own_rec + (((uint64_t)u0 * kvh + head / g) * g + head % g) * kRecord;
-  const uint64_t ostep = (uint64_t)kvh * g * kRecord;
-  auto record = [&](uint32_t i) { return i < np ? pp + (uint64_t)i * kRecord : po + (i - np) * ostep; };
-  float M = -__builtin_inff();
-  for (uint32_t i = lane; i < n; i += 64) M = fmaxf(M, record(i)[0]);
-  M = wave_max(M);
-  float L = 0.f, n0 = 0.f, n1 = 0.f;
-  for (uint32_t c0 = 0; c0 < n; c0 += 64) {
-    const uint32_t mine = min(c0 + lane, n - 1);
-    const float w = c0 + lane < n ? __builtin_amdgcn_exp2f(record(mine)[0] - M) : 0.f;
-    const float lw = w * record(mine)[1];
-    L += wave_sum(lw);
-    const uint32_t cn = min(64u, n - c0);
-    for (uint32_t s0 = 0; s0 < cn; s0 += 8) {
-      float a0[8], a1[8];
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const float2 v = *reinterpret_cast<const float2*>(record(c0 + min(s0 + u, cn - 1)) + 4 + 2 * lane);
-        a0[u] = v.x;
-        a1[u] = v.y;
-      }
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const float f = s0 + u < cn ? lane_bcast(w, (int)(s0 + u)) : 0.f;
-        n0 = __builtin_fmaf(a0[u], f, n0);
-        n1 = __builtin_fmaf(a1[u], f, n1);
-      }
-    }
-  }
-  const uint32_t o0 = f32_to_bf16(n0 / L), o1 = f32_to_bf16(n1 / L);
-  const uint32_t col = head * 128 + 2 * lane;
-  uint16_t* dst = out_mtiles ? out + act_offset_m(r, col, out_mtiles) : out + (uint64_t)r * qh * 128 + col;
-  *reinterpret_cast<uint32_t*>(dst) = o0 | (o1 << 16);
-  if (!(L > 0.f) || ((o0 & 0x7f80u) == 0x7f80u) || ((o1 & 0x7f80u) == 0x7f80u)) raise_error(err, ERR_NONFINITE);
-}
-
-// The launch's work split: a rule on the groups, heads and lengths alone, so
+// The launches' work split: a rule on the groups, heads and numbers of rows alone, so
 // that the scratch's size and the launch agree.
 struct PrefixPlan {
   Groups gs;
-  uint32_t items, form, own_wgs;
-  uint64_t prefix_floats, own_floats;  // of the records
+  uint32_t items, form, max_parts, counters;
+  uint64_t prefix_floats, part_floats;  // of the records
 };
 
 PrefixPlan prefix_plan(const fh_prefix_group* groups, uint32_t ngroups, uint32_t rows, uint32_t qh, uint32_t kvh) {
@@ -673,13 +695,13 @@ PrefixPlan prefix_plan(const fh_prefix_group* groups, uint32_t ngroups, uint32_t
     if (to.rows > most) most = to.rows;
   }
   const uint64_t vectors = (uint64_t)most * g;
-  p.form = vectors > 64 ? 1 : vectors > 16 ? 2 : 0;
-  p.gs.block_rows = (p.form == 1 ? 128 : p.form == 2 ? 64 : 16) / g;
-  // Two workgroups per CU over the prefixes, of at least kMinChunk tokens.
+  p.form = vectors > 64 ? 1 : vectors > kVectors ? 2 : 0;
+  p.gs.block_rows = (p.form == 1 ? 128 : p.form == 2 ? 64 : kVectors) / g;
+  // About two workgroups per CU, of at least kMinChunk tokens.
   uint64_t tokens = 0;
   for (uint32_t i = 0; i < p.gs.count; ++i)
     tokens += (uint64_t)p.gs.g[i].prefix_tokens * ((p.gs.g[i].rows + p.gs.block_rows - 1) / p.gs.block_rows) * kvh;
-  uint64_t chunk = (tokens / 512 + kKeys - 1) / kKeys * kKeys;
+  uint64_t chunk = (tokens / kSlots + 63) / 64 * 64;
   if (chunk < kMinChunk) chunk = kMinChunk;
   p.gs.chunk = (uint32_t)chunk;
   for (uint32_t i = 0; i < p.gs.count; ++i) {
@@ -689,10 +711,12 @@ PrefixPlan prefix_plan(const fh_prefix_group* groups, uint32_t ngroups, uint32_t
     p.items += chunks * ((to.rows + p.gs.block_rows - 1) / p.gs.block_rows);
     if (chunks > p.gs.prefix_slots) p.gs.prefix_slots = chunks;
   }
-  p.own_wgs = kOwnWgs;
+  // Parts of the own keys: what fills the slots; one where the rows and heads do.
+  const uint64_t pairs = (uint64_t)rows * kvh;
+  p.max_parts = pairs >= kSlots ? 1 : (uint32_t)(kSlots / pairs) < kMaxParts ? (uint32_t)(kSlots / pairs) : kMaxParts;
+  p.counters = p.max_parts > 1 ? (uint32_t)pairs : 0;
   p.prefix_floats = (uint64_t)rows * qh * p.gs.prefix_slots * kRecord;
-  // Units: a row's last one may be short, the others hold at least all / kOwnUnits pages and heads.
-  p.own_floats = ((uint64_t)kOwnUnits + kvh + (uint64_t)rows * kvh) * g * kRecord;
+  p.part_floats = p.max_parts > 1 ? (uint64_t)rows * qh * p.max_parts * kRecord : 0;
   return p;
 }
 
@@ -700,7 +724,7 @@ PrefixPlan prefix_plan(const fh_prefix_group* groups, uint32_t ngroups, uint32_t
 
 uint64_t prefix_scratch_bytes(const fh_prefix_group* groups, uint32_t ngroups, uint32_t rows, uint32_t qh, uint32_t kvh) {
   const PrefixPlan p = prefix_plan(groups, ngroups, rows, qh, kvh);
-  return (p.prefix_floats + p.own_floats + rows + 1) * 4;
+  return (p.prefix_floats + p.part_floats + p.counters + 4) * 4;  // never nothing
 }
 
 hipError_t launch_prefix_attention(const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache,
@@ -710,21 +734,26 @@ hipError_t launch_prefix_attention(const uint16_t* q, const uint16_t* k_cache, c
                                    uint32_t* err, hipStream_t s) {
   const PrefixPlan p = prefix_plan(groups, ngroups, rows, qh, kvh);
   float* prefix_rec = reinterpret_cast<float*>(scratch);
-  float* own_rec = prefix_rec + p.prefix_floats;
-  uint32_t* first = reinterpret_cast<uint32_t*>(own_rec + p.own_floats);
-  const uint32_t prefix_wgs = p.items * kvh;
+  float* part_rec = prefix_rec + p.prefix_floats;
+  uint32_t* counters = reinterpret_cast<uint32_t*>(part_rec + p.part_floats);
   const Args a{q, k_cache, v_cache, qh, kvh, pages, err};
-#define FH_PREFIX_FORM(G_, FORM_)                                                                                 \
-  hipLaunchKernelGGL((prefix_kernel<G_, FORM_>), dim3(prefix_wgs + p.own_wgs), dim3(kThreads), 0, s, a, positions, \
-                     table, rows, stride, context, prefix_wgs, p.own_wgs, prefix_rec, own_rec, first, p.gs)
-#define FH_PREFIX(G_)            \
-  do {                           \
-    if (p.form == 1)             \
-      FH_PREFIX_FORM(G_, 1);     \
-    else if (p.form == 2)        \
-      FH_PREFIX_FORM(G_, 2);     \
-    else                         \
-      FH_PREFIX_FORM(G_, 0);     \
+  const uint32_t mt = out_tiled ? act_mtiles(rows) : 0u;
+  const uint32_t prefix_wgs = p.items ? p.items * kvh : p.counters ? 1 : 0;
+#define FH_PREFIX_FORM(G_, FORM_)                                                                                      \
+  hipLaunchKernelGGL((prefix_kernel<G_, FORM_>), dim3(prefix_wgs), dim3(kThreads), 0, s, a, table, stride, p.items, \
+                     prefix_rec, counters, p.counters, p.gs)
+#define FH_PREFIX(G_)                                                                                               \
+  do {                                                                                                              \
+    if (prefix_wgs) {                                                                                               \
+      if (p.form == 1)                                                                                              \
+        FH_PREFIX_FORM(G_, 1);                                                                                      \
+      else if (p.form == 2)                                                                                         \
+        FH_PREFIX_FORM(G_, 2);                                                                                      \
+      else                                                                                                          \
+        FH_PREFIX_FORM(G_, 0);                                                                                      \
+    }                                                                                                               \
+    hipLaunchKernelGGL((own_kernel<G_>), dim3(kvh * rows * p.max_parts), dim3(kThreads), 0, s, a, positions, table, \
+                       rows, stride, context, p.max_parts, prefix_rec, part_rec, counters, out, mt, p.gs);          \
   } while (0)
   switch (qh / kvh) {
     case 1: FH_PREFIX(1); break;
@@ -735,11 +764,6 @@ hipError_t launch_prefix_attention(const uint16_t* q, const uint16_t* k_cache, c
   }
 #undef FH_PREFIX
 #undef FH_PREFIX_FORM
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  const uint64_t waves = (uint64_t)rows * qh;
-  hipLaunchKernelGGL(prefix_merge_kernel, dim3((waves + 3) / 4), dim3(256), 0, s, prefix_rec, own_rec, first, positions,
-                     out, out_tiled ? act_mtiles(rows) : 0u, rows, qh, kvh, stride, context, err, p.gs);
   return hipGetLastError();
 }
 

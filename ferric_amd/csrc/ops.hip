@@ -423,7 +423,7 @@ fh_status fh_op_prefix_attention(const uint16_t* q, const uint16_t* k_cache, con
   if (!q || !k_cache || !v_cache || !positions || !page_table || !out || !scratch || stride == 0 ||
       physical_pages == 0 || (uint64_t)stride * 16 < context_tokens ||
       !prefix_shape_ok(rows, query_heads, kv_heads, context_tokens) || !aligned(q, 16) || !aligned(k_cache, 16) ||
-      !aligned(v_cache, 16) || !aligned(out, 4) || !aligned(scratch, 16))
+      !aligned(v_cache, 16) || !aligned(out, 8) || !aligned(scratch, 16))
     return FH_ERR_INVALID_ARGUMENT;
   if (const char* why = fh::prefix_groups_refused(groups, ngroups, rows, context_tokens)) {
     fh::set_thread_error(why);

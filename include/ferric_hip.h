@@ -429,7 +429,7 @@ typedef struct fh_prefix_group {
  * position >= 16 x prefix_pages - 1 (its prefix is all visible; ERR_POSITION in error_word
  * and no output for the row otherwise), and its table's first prefix_pages entries are those
  * of the group's first row (the page bit of error_word otherwise). q, out, out_tiled, tables
- * and errors as fh_op_paged_attention; q and the caches 16-byte, out 4-byte aligned. scratch:
+ * and errors as fh_op_paged_attention; q and the caches 16-byte, out 8-byte aligned. scratch:
  * fh_prefix_attention_scratch_bytes() of the same arguments, 16-byte aligned, for this call
  * alone until it has run. Rows with one or several query heads per KV head (1, 2, 4, 8). FP32
  * reassociation: the states of chunks of keys are merged, so the result differs from

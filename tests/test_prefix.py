@@ -47,7 +47,7 @@ def test_more_groups_than_a_launch_holds_are_refused():
                                  dict(scratch=None), dict(rows=0, groups=groups_of()), dict(rows=65536), dict(context=2**24 + 16, stride=2**21), dict(qh=31),
                                  dict(qh=24), dict(qh=128), dict(kvh=0), dict(stride=7), dict(stride=0), dict(pages=0),
                                  dict(context=0, groups=groups_of()), dict(q=P + 8), dict(k=P + 8), dict(v=P + 8),
-                                 dict(out=P + 2), dict(scratch=P + 4), dict(nbytes=100)])
+                                 dict(out=P + 4), dict(scratch=P + 4), dict(nbytes=100)])
 def test_shapes_and_pointers_that_are_refused(bad):
     assert call(**bad) == 1
 
