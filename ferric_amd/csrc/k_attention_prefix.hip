@@ -8,8 +8,9 @@
 // states over each: with (m_i, l_i, n_i) = (max s, sum e^(s - m_i), sum
 // e^(s - m_i) v), M = max m_i, out = sum n_i e^(m_i - M) / sum l_i e^(m_i - M).
 // A state covers a chunk of a prefix (for up to 128 query vectors of one KV head
-// at once) or a unit of a row's own keys; states are FP32 records in the
-// scratch, merged in ascending key order by a second launch.
+// at once) or a part of a row's own keys. Two launches: the first leaves the
+// chunks' states as FP32 records in the scratch; the second takes the own keys and
+// joins them with the records.
 //
 // A wave owns 16 query vectors (vector j: row j / G, head j % G of the KV head)
 // and walks keys 32 or 64 at a time:
@@ -30,12 +31,24 @@
 // at c ^ 2 (t % 8). Slots that are no keys of the state are outside the loads'
 // buffer bounds and arrive as zeros, so what they hold never meets an MFMA.
 //
-// Two forms share the launch. Wide (prefix chunks of more than 16 vectors): the 8
-// waves share 64-key tiles of K and V, fetched global -> LDS directly, double-
-// buffered; 8 waves of vectors, or 4 with two of them sharing the tile's keys.
-// Narrow (own keys, and prefix chunks of up to 16 vectors): the waves take 32 keys
-// each, K straight into the A operand's registers (a token's 64-byte pieces), V
-// through 8 KiB of LDS of the wave's own; their states meet in LDS at the end.
+// Forms. Wide (prefix chunks of more than 16 vectors): the 8 waves share 64-key
+// tiles of K and V, fetched global -> LDS directly, double-buffered: all 8 with
+// vectors of their own (128 a workgroup), or 4 pairs of waves (64 vectors) of which
+// each takes half of a tile's keys, which halves the time from a tile's arrival to
+// the next fetch. Narrow (own keys, and prefix chunks of up to 16 vectors): the waves
+// take 32 keys each, K straight into the A operand's registers (a token's 64-byte
+// pieces), V through 8 KiB of LDS of the wave's own; their states meet in LDS at the
+// end. All forms keep to 128 registers a thread and 67.6 KB of LDS, so that two
+// workgroups share a CU and one computes while the other waits.
+//
+// What bounds it (kernel times, 32 rows, 8 KV heads of 4 query heads): behind 8192
+// shared tokens the first launch takes 15 us (33.6 MB of keys and values, which the
+// 256 MB cache keeps between steps, and 17 MB of records) and the second 12, a
+// chain of latencies: position -> records -> page table -> keys -> join. Behind
+// 32000 tokens the first takes 38: 131 MB from HBM at 3.5 TB/s, from the bytes that
+// two tiles a workgroup keep in flight. One workgroup a CU with four tiles in flight
+// was slower (18 us and 42): its waves then wait for one another at every tile with
+// nothing else on the CU.
 #include <type_traits>
 
 #include "common.hpp"
@@ -54,8 +67,20 @@ constexpr int kThreads = 64 * kWaves;
 constexpr int kKeys = 64;             // keys per tile of the wide form
 constexpr int kStep = 32 * kWaves;    // keys of the narrow form's waves at once
 constexpr size_t kTileBytes = 16 * 2 * kKeys * 16;  // K or V, double-buffered
-constexpr uint32_t kMinChunk = 256;   // least tokens of a prefix chunk
-constexpr uint32_t kPartKeys = 512;   // least own keys of a part where a row has several
+// Least tokens of a prefix chunk (256 instead: 4 rows behind 1488 tokens 1.1 us slower).
+constexpr uint32_t kMinChunk = 128;
+// Chunks are cut for about this many workgroups: more of them write and join more records, fewer
+// leave CUs idle (32 rows behind 8192 tokens: 26.4 us with 256; 192 and 384 were slower in every case tried).
+constexpr uint32_t kChunkWgs = 256;
+// From this many bytes of prefix that one pass reads once each it streams past the caches (32 rows
+// behind 32000 tokens, 131 MB: 61.7 us cached, 53.2 streamed; smaller ones, which the
+// 256 MB cache still holds from the step before, are 3 to 10 % slower streamed).
+constexpr uint64_t kStreamBytes = 96ull << 20;
+// Least own keys of a part where a row has several. A step of kStep keys takes about 3.5 us and the
+// meeting of the parts about 3: with few (row, KV head) pairs 256 (2 rows of 2000 own keys:
+// 18.9 us, with 512 21.0, with 1024 29.4), with many, where parts only take turns, 512
+// (29 rows of up to 900: 25.8 us with 256, 24.5 with 512).
+constexpr uint32_t kPartKeysFew = 256, kPartKeysMany = 512, kManyPairs = 128;
 constexpr uint32_t kMaxParts = 32;
 constexpr uint32_t kSlots = 512;      // workgroups that run at once: two on each CU
 constexpr uint32_t kVectors = 16;     // of a wave
@@ -68,7 +93,7 @@ struct Group {
   uint32_t item0;  // its first prefix item: vector block + blocks * chunk
 };
 struct Groups {
-  uint32_t count, chunk, block_rows, prefix_slots;
+  uint32_t count, chunk, block_rows, prefix_slots, stream;
   Group g[kPrefixMaxGroups];
 };
 
@@ -118,7 +143,8 @@ struct State {
     for (int d = 0; d < 8; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  // Takes in T tiles of 16 scores: keys first + 16 t + 4 (lane / 16) + e below `end`. v_at(t, d, v): the V^T operands of tiles t, t + 1 (t even) for dims 16 d .. + 63.
+  // Takes in T tiles of 16 scores: keys first + 16 t + 4 (lane / 16) + e below `end`.
+  // v_at(t, d, v): the V^T operands of tiles t, t + 1 (t even) for dims 16 d .. + 63.
   template <int T, class V>
   __device__ __forceinline__ void take(f32x4 (&s)[T], uint32_t first, uint32_t end, const V& v_at) {
     const float kNegInf = -__builtin_inff();
@@ -280,7 +306,7 @@ __device__ __forceinline__ Page page_of(const Args& a, uint32_t page, uint32_t v
 template <int G, int WK>
 __device__ __forceinline__ void attend_wide(unsigned char* lds_raw, const Args& a, const uint32_t* __restrict__ trow,
                                             uint32_t row0, uint32_t nrows, uint32_t key0, uint32_t key1, uint32_t h,
-                                            float* rec, uint32_t slots) {
+                                            bool stream, float* rec, uint32_t slots) {
   constexpr int WQ = kWaves / WK, kTiles = kKeys / 16 / WK;  // 16-key tiles a wave takes of each 64
   auto& klds = *reinterpret_cast<u32x4(*)[2][kKeys][16]>(lds_raw);
   auto& vlds = *reinterpret_cast<u32x4(*)[2][kKeys][16]>(lds_raw + kTileBytes);
@@ -305,11 +331,15 @@ __device__ __forceinline__ void attend_wide(unsigned char* lds_raw, const Args& 
     const uint32_t page = (uint32_t)__builtin_amdgcn_readlane((int)tab, (int)(pi & 63u));
     const Page p = page_of(a, page, pi < npages ? min(16u, key1 - key0 - pi * 16) : 0u, h, bad_page);
     auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)((is_v ? a.vc : a.kc) + p.base), 0, p.bytes, 0x00020000);
-    u32x4(*to)[16] = (is_v ? vlds : klds)[t & 1];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          rsrc, (__attribute__((address_space(3))) void*)&to[16 * my_page + 4 * i][0], 16, off[i], 0, 0, 0);
+    u32x4(*to)[16] = (is_v ? vlds : klds)[t & 1] + 16 * my_page;
+#define FH_FETCH(AUX_)                                                                                             \
+  _Pragma("unroll") for (int i = 0; i < 4; ++i) __builtin_amdgcn_raw_ptr_buffer_load_lds(                          \
+      rsrc, (__attribute__((address_space(3))) void*)&to[4 * i][0], 16, off[i], 0, 0, AUX_)
+    if (stream)
+      FH_FETCH(2);  // non-temporal
+    else
+      FH_FETCH(0);
+#undef FH_FETCH
   };
   fetch(0);
   const uint32_t vec = kVectors * wq + (lane & 15);
@@ -386,11 +416,39 @@ __device__ __forceinline__ void attend_wide(unsigned char* lds_raw, const Args& 
   if (bad_page != 0 && lane == 0) raise_error(a.err, ERR_PAGE);
 }
 
-// LDS of the narrow form: V of each wave's 32 keys, then the waves' states.
-struct NarrowState {
-  float acc[kWaves][kVectors][128];
+// A state over some keys: the vector's maximum (in the exponent of 2), its sum and four of its dims.
+struct Part {
+  float m, l;
+  f32x4 n;
 };
-static_assert(sizeof(NarrowState) == 2 * kTileBytes, "the states of 8 waves fill the tiles' LDS");
+__device__ __forceinline__ Part no_part() { return Part{-__builtin_inff(), 0.f, f32x4{0.f, 0.f, 0.f, 0.f}}; }
+// The union's state with N more: their maximum, then one sum. (One without keys has m = -inf and l = 0.)
+template <int N>
+__device__ __forceinline__ Part join_all(const Part& t, const Part (&x)[N]) {
+  const float kNegInf = -__builtin_inff();
+  float m = t.m;
+#pragma unroll
+  for (int u = 0; u < N; ++u) m = fmaxf(m, x[u].m);
+  const float f = t.m == kNegInf ? 0.f : __builtin_amdgcn_exp2f(t.m - m);
+  Part o{m, t.l * f, t.n};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o.n[e] *= f;
+#pragma unroll
+  for (int u = 0; u < N; ++u) {
+    const float w = x[u].m == kNegInf ? 0.f : __builtin_amdgcn_exp2f(x[u].m - m);
+    o.l = __builtin_fmaf(x[u].l, w, o.l);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o.n[e] = __builtin_fmaf(x[u].n[e], w, o.n[e]);
+  }
+  return o;
+}
+
+// LDS of the narrow form: V of each wave's 32 keys, then the waves' states.
+// (Rows of 528 bytes keep the accumulators' stores off each other's banks.)
+struct NarrowState {
+  float acc[kWaves][kVectors][132];
+};
+static_assert(sizeof(NarrowState) >= 2 * kTileBytes, "and the wide form's tiles fit too");
 struct NarrowSums {
   float m[kWaves][kVectors], l[kWaves][kVectors];  // m in the exponent of 2
 };
@@ -481,23 +539,6 @@ __device__ __forceinline__ void attend_narrow(unsigned char* lds_raw, NarrowSums
   __syncthreads();
 }
 
-// A state over some keys: the vector's maximum (in the exponent of 2), its sum and four of its dims.
-struct Part {
-  float m, l;
-  f32x4 n;
-};
-__device__ __forceinline__ Part no_part() { return Part{-__builtin_inff(), 0.f, f32x4{0.f, 0.f, 0.f, 0.f}}; }
-// The union's state. (One without keys has m = -inf and l = 0.)
-__device__ __forceinline__ Part join(const Part& x, const Part& y) {
-  const float m = fmaxf(x.m, y.m);
-  const float fx = x.m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(x.m - m);
-  const float fy = y.m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(y.m - m);
-  Part o{m, x.l * fx + y.l * fy, f32x4{0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-  for (int e = 0; e < 4; ++e) o.n[e] = x.n[e] * fx + y.n[e] * fy;
-  return o;
-}
-
 // The waves' states of vector v, dims 4 c .. 4 c + 3, joined in wave order (the maximum first, then one sum).
 __device__ __forceinline__ Part narrow_part(unsigned char* lds_raw, const NarrowSums& sums, uint32_t v, uint32_t c) {
   auto& all = *reinterpret_cast<NarrowState*>(lds_raw);
@@ -528,7 +569,7 @@ template <int G, int FORM>
 __global__ __launch_bounds__(kThreads, 4) void prefix_kernel(Args a, const uint32_t* __restrict__ table, uint32_t stride,
                                                              uint32_t items, float* rec, uint32_t* counters,
                                                              uint32_t ncounters, Groups gs) {
-  __shared__ __attribute__((aligned(16))) unsigned char lds_raw[2 * kTileBytes];
+  __shared__ __attribute__((aligned(16))) unsigned char lds_raw[sizeof(NarrowState)];
   const uint32_t h = blockIdx.x % a.kvh, item = blockIdx.x / a.kvh;
   if (blockIdx.x == 0 && threadIdx.x < ncounters) counters[threadIdx.x] = 0u;
   if (item >= items) return;
@@ -553,7 +594,7 @@ __global__ __launch_bounds__(kThreads, 4) void prefix_kernel(Args a, const uint3
       if (c == 0) *reinterpret_cast<float2*>(r) = make_float2(o.m, o.l);
     }
   } else {
-    attend_wide<G, FORM>(lds_raw, a, trow, row0, nrows, key0, key1, h, rec, gs.prefix_slots);
+    attend_wide<G, FORM>(lds_raw, a, trow, row0, nrows, key0, key1, h, gs.stream != 0, rec, gs.prefix_slots);
   }
   if (h == 0) {
     // The rows of the block list the same pages here as the group's first row.
@@ -567,7 +608,7 @@ __global__ __launch_bounds__(kThreads, 4) void prefix_kernel(Args a, const uint3
 }
 
 // Second launch: (KV head, row, part) takes a part of the row's own keys, which are
-// cut into at most `parts` equal ones of at least kPartKeys keys, and the first part
+// cut into at most max_parts equal ones of at least part_keys keys, and the first part
 // the records of the prefix's chunks too. A row of one part ends here; the parts
 // of longer ones leave records, and the last one to arrive (a counter per row and KV
 // head, which the first launch cleared) joins them in key order. Records and counter
@@ -581,16 +622,15 @@ template <int G>
 __global__ __launch_bounds__(kThreads, 4) void own_kernel(Args a, const uint32_t* __restrict__ positions,
                                                           const uint32_t* __restrict__ table, uint32_t rows,
                                                           uint32_t stride, uint32_t context, uint32_t max_parts,
+                                                          uint32_t part_keys,
                                                           const float* __restrict__ prefix_rec, float* part_rec,
                                                           uint32_t* counters, uint16_t* __restrict__ out,
                                                           uint32_t out_mtiles, Groups gs) {
   constexpr uint32_t kDims = G * 32;                // (vector, four dims) pairs
   constexpr uint32_t kTeams = kThreads / kDims;     // threads per pair, for the prefix's records
   constexpr int kInFlight = 4;
-  __shared__ __attribute__((aligned(16))) unsigned char lds_raw[2 * kTileBytes];
+  __shared__ __attribute__((aligned(16))) unsigned char lds_raw[sizeof(NarrowState)];
   __shared__ NarrowSums sums;
-  __shared__ f32x4 team_n[kTeams][kDims];
-  __shared__ float team_m[kTeams][G], team_l[kTeams][G];
   const uint32_t h = blockIdx.x % a.kvh, r = blockIdx.x / a.kvh % rows, part = blockIdx.x / a.kvh / rows;
   const uint32_t pos = uniform(positions[r]), prefix = prefix_of(gs, r);
   if (pos >= context || pos / 16 >= stride || pos + 1 < prefix) {
@@ -598,16 +638,18 @@ __global__ __launch_bounds__(kThreads, 4) void own_kernel(Args a, const uint32_t
     return;
   }
   const uint32_t own = pos + 1 - prefix;
-  const uint32_t wanted = max(1u, min(max_parts, own / kPartKeys));
+  const uint32_t wanted = max(1u, min(max_parts, own / part_keys));
   const uint32_t keys = (own + wanted * kStep - 1) / (wanted * kStep) * kStep;  // of a part
   const uint32_t parts = own > keys ? (own + keys - 1) / keys : 1u;
   if (part >= parts) return;
   const uint32_t v = threadIdx.x % kDims / 32, c = threadIdx.x % 32, team = threadIdx.x / kDims;
-  if (part == 0) {
-    // The prefix's chunks, every kTeams-th one, kInFlight records at a time.
-    Part t = no_part();
-    const uint32_t chunks = (prefix + gs.chunk - 1) / gs.chunk;
+  __shared__ f32x4 team_n[kThreads];
+  __shared__ float2 team_ml[kTeams][G];
+  const uint32_t chunks = part == 0 ? (prefix + gs.chunk - 1) / gs.chunk : 0u;
+  if (chunks) {
+    // The records of the prefix's chunks, every kTeams-th one, kInFlight at a time: their maximum, then one sum.
     const float* p = prefix_rec + ((uint64_t)r * a.qh + h * G + v) * gs.prefix_slots * kRecord;
+    Part t = no_part();
     for (uint32_t i0 = team; i0 < chunks; i0 += kTeams * kInFlight) {
       Part x[kInFlight];
 #pragma unroll
@@ -618,23 +660,25 @@ __global__ __launch_bounds__(kThreads, 4) void own_kernel(Args a, const uint32_t
       }
 #pragma unroll
       for (int u = 0; u < kInFlight; ++u)
-        if (i0 + u * kTeams < chunks) t = join(t, x[u]);
+        if (i0 + u * kTeams >= chunks) x[u].m = -__builtin_inff();
+      t = join_all(t, x);
     }
-    team_n[team][threadIdx.x % kDims] = t.n;
-    if (c == 0) {
-      team_m[team][v] = t.m;
-      team_l[team][v] = t.l;
-    }
+    team_n[threadIdx.x] = t.n;
+    if (c == 0) team_ml[team][v] = make_float2(t.m, t.l);
   }
   const uint32_t key0 = prefix + part * keys, key1 = min(key0 + keys, pos + 1);
   attend_narrow<G>(lds_raw, sums, a, table + (uint64_t)r * stride, r, 1, key0, key1, h);
   const bool mine = threadIdx.x < kDims;
   Part o = no_part();
   if (mine) {
-    if (part == 0)
+    o = narrow_part(lds_raw, sums, v, c);
+    if (chunks) {
+      Part x[kTeams];
 #pragma unroll
-      for (uint32_t t = 0; t < kTeams; ++t) o = join(o, Part{team_m[t][v], team_l[t][v], team_n[t][threadIdx.x]});
-    o = join(o, narrow_part(lds_raw, sums, v, c));
+      for (uint32_t t = 0; t < kTeams; ++t)
+        x[t] = Part{team_ml[t][v].x, team_ml[t][v].y, team_n[t * kDims + threadIdx.x]};
+      o = join_all(o, x);
+    }
   }
   if (parts > 1) {
     __shared__ uint32_t last;
@@ -658,12 +702,13 @@ __global__ __launch_bounds__(kThreads, 4) void own_kernel(Args a, const uint32_t
       o = no_part();
       for (uint32_t i = 0; i < parts; ++i) {
         const float* x = to + (uint64_t)i * G * kRecord;
-        Part y;
-        y.m = __hip_atomic_load(x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        y.l = __hip_atomic_load(x + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        Part y[1];
+        y[0].m = __hip_atomic_load(x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        y[0].l = __hip_atomic_load(x + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y.n[e] = __hip_atomic_load(x + 4 + 4 * c + e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        o = join(o, y);
+        for (int e = 0; e < 4; ++e)
+          y[0].n[e] = __hip_atomic_load(x + 4 + 4 * c + e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        o = join_all(o, y);
       }
     }
   }
@@ -680,7 +725,7 @@ __global__ __launch_bounds__(kThreads, 4) void own_kernel(Args a, const uint32_t
 // that the scratch's size and the launch agree.
 struct PrefixPlan {
   Groups gs;
-  uint32_t items, form, max_parts, counters;
+  uint32_t items, form, max_parts, part_keys, counters;
   uint64_t prefix_floats, part_floats;  // of the records
 };
 
@@ -695,13 +740,22 @@ PrefixPlan prefix_plan(const fh_prefix_group* groups, uint32_t ngroups, uint32_t
     if (to.rows > most) most = to.rows;
   }
   const uint64_t vectors = (uint64_t)most * g;
-  p.form = vectors > 64 ? 1 : vectors > kVectors ? 2 : 0;
+  if (most == 0) most = 1;
+  // Tokens times blocks times KV heads with blocks of `rows` rows.
+  auto tokens_of = [&](uint32_t rows) {
+    uint64_t tokens = 0;
+    for (uint32_t i = 0; i < p.gs.count; ++i)
+      tokens += (uint64_t)p.gs.g[i].prefix_tokens * ((p.gs.g[i].rows + rows - 1) / rows) * kvh;
+    return tokens;
+  };
+  // Blocks of 64 vectors unless the prefixes are long: 32 rows of 4 heads behind 8192 tokens 26.4 us
+  // (29.8 in blocks of 128, whose waves take whole tiles), but 160 rows behind 4096 tokens 49.7 us (47.5 in
+  // blocks of 128, which read the keys half as often) and 32 behind 32000 69.4 (61.7).
+  p.form = vectors > kVectors ? 2 : 0;
+  if (vectors > 64 && tokens_of(128 / g) / kChunkWgs >= 512) p.form = 1;
   p.gs.block_rows = (p.form == 1 ? 128 : p.form == 2 ? 64 : kVectors) / g;
-  // About two workgroups per CU, of at least kMinChunk tokens.
-  uint64_t tokens = 0;
-  for (uint32_t i = 0; i < p.gs.count; ++i)
-    tokens += (uint64_t)p.gs.g[i].prefix_tokens * ((p.gs.g[i].rows + p.gs.block_rows - 1) / p.gs.block_rows) * kvh;
-  uint64_t chunk = (tokens / kSlots + 63) / 64 * 64;
+  p.gs.stream = most <= p.gs.block_rows && tokens_of(most) * 512 >= kStreamBytes;
+  uint64_t chunk = (tokens_of(p.gs.block_rows) / kChunkWgs + 63) / 64 * 64;
   if (chunk < kMinChunk) chunk = kMinChunk;
   p.gs.chunk = (uint32_t)chunk;
   for (uint32_t i = 0; i < p.gs.count; ++i) {
@@ -714,6 +768,7 @@ PrefixPlan prefix_plan(const fh_prefix_group* groups, uint32_t ngroups, uint32_t
   // Parts of the own keys: what fills the slots; one where the rows and heads do.
   const uint64_t pairs = (uint64_t)rows * kvh;
   p.max_parts = pairs >= kSlots ? 1 : (uint32_t)(kSlots / pairs) < kMaxParts ? (uint32_t)(kSlots / pairs) : kMaxParts;
+  p.part_keys = pairs > kManyPairs ? kPartKeysMany : kPartKeysFew;
   p.counters = p.max_parts > 1 ? (uint32_t)pairs : 0;
   p.prefix_floats = (uint64_t)rows * qh * p.gs.prefix_slots * kRecord;
   p.part_floats = p.max_parts > 1 ? (uint64_t)rows * qh * p.max_parts * kRecord : 0;
@@ -753,7 +808,8 @@ hipError_t launch_prefix_attention(const uint16_t* q, const uint16_t* k_cache, c
         FH_PREFIX_FORM(G_, 0);                                                                                      \
     }                                                                                                               \
     hipLaunchKernelGGL((own_kernel<G_>), dim3(kvh * rows * p.max_parts), dim3(kThreads), 0, s, a, positions, table, \
-                       rows, stride, context, p.max_parts, prefix_rec, part_rec, counters, out, mt, p.gs);          \
+                       rows, stride, context, p.max_parts, p.part_keys, prefix_rec, part_rec, counters, out, mt,    \
+                       p.gs);                                                                                       \
   } while (0)
   switch (qh / kvh) {
     case 1: FH_PREFIX(1); break;
