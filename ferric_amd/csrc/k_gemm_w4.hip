@@ -6,24 +6,32 @@
 // with q in 0..15, groups of 32, 64 or 128 consecutive columns, bf16 scales s
 // and zero points z (8 where none are given).
 //
-// A 4-bit weight enters the MFMA as the bf16 number 128 + q, which is exact (8
-// significant bits: 128..143) and one and-or for two weights: the nibble is the
-// low end of the mantissa of 0x4300. The 128 and the zero point come off per
-// group, in FP32: sum (q - z) x = sum (128 + q) x - (128 + z) sum x, where sum x
-// is the MFMA of the activations with a tile of ones, shared by the wave's
-// weight tiles. The subtraction cancels: the terms are up to 136 / 7 of what is
-// left, so the group's sum carries about 20 roundings' worth of FP32 error
-// (2e-6 relative to a group's result), 1/2000 of the bf16 output's.
+// A 4-bit weight enters the MFMA as the bf16 number 16 + q, which is exact, from
+// a shift and an and-or for two weights: the nibble is the top of the mantissa of
+// 0x4180. The 16 comes off in the accumulators, which start a group as the MFMA of
+// its activations with a tile of -16 (of -24 where there are no zero points: the 8
+// with it); that, -16 sum x in every column, serves the zero points too:
+// sum (q - z) x = [sum (16 + q) x - 16 sum x] + z / 16 (-16 sum x). The weight tiles
+// of a wave share it. What cancels is at most 31 / 4.6 of what is left (root mean
+// squares), so a group's FP32 roundings count up to seven times: the error measured
+// is 9e-8 of the result's norm, against 8e-7 with 128 + q (one shift less) in its place.
 //
 // Layout (fh_op_tile_weight_w4): a 16-row x 128-column tile is 1 KiB, one
 // 16-byte load per lane; lane = row + 16 (column % 32 / 8), its four words are
-// the four 32-column k-blocks, so word j is the A operand of k-block j's MFMA
+// the four 32-column k-blocks, so word j is the B operand of k-block j's MFMA
 // before unpacking: columns 2 i and 2 i + 1 of a word's eight at bits 4 i and
-// 16 + 4 i, which (word >> 4 i) & 0x000f000f takes out as a pair. Tiles run
-// k-fastest. Scales and zero points: [n / 16][groups][16], so the four rows of
-// a lane's accumulators are one 8-byte (4-byte) load. Activations in their tile
-// order (common.hpp act_offset). Lanes of rows past m read the last row again
-// (less to fetch; their output columns are not stored).
+// 16 + 4 i, so that a shift and 0x00780078 take out a pair. Tiles run k-fastest. Scales
+// and zero points: [n / 16][groups][16]; a tile's are one load each, a lane's being
+// its row's and those of one group of the 128 columns. Activations in their tile
+// order (common.hpp act_offset) are the A operand. Lanes of rows past m read the
+// last row again (less to fetch; their output rows are not stored).
+//
+// What bounds it: the weights' bytes from HBM in 7 rows through 151936 x 4096 (60
+// us, 325 MB at 5.4 TB/s, the rate of a large copy); a launch's start and end beside them
+// in one row through 24576 x 4096 (12.3 us, 52 MB; 9.6 at that rate). From about 16
+// rows on, and with few weight rows a workgroup, the activations, which every workgroup
+// reads whole from the L2: 32 rows through 4096 x 12288 take 786 KB into each CU
+// beside 115 KB of weights, 16.2 us, and 10.8 with those loads left out.
 #include "common.hpp"
 #include "kernels.hpp"
 
@@ -33,24 +41,34 @@ namespace {
 
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ bf16x8 unpack_w4(uint32_t w) {
-  // Eight nibbles to bf16 128 + q.
-  const u32x4 v = {(w & 0x000f000fu) | 0x43004300u, ((w >> 4) & 0x000f000fu) | 0x43004300u,
-                   ((w >> 8) & 0x000f000fu) | 0x43004300u, ((w >> 12) & 0x000f000fu) | 0x43004300u};
+// Waves of a workgroup, which divide its k: 4 where there are kMany workgroups (one row through 24576 x 4096
+// in 768 of them: 12.2 us, 13.1 with 16 waves, 14.7 with 8), else 16 (4 rows through 4096 x 4096 in 256: 4.7 us,
+// 5.7 with 8, 8.6 with 4; 1024 x 2048 in 64: 2.9, 3.0, 3.6).
+constexpr uint32_t kMany = 512;
+constexpr int kWavesFew = 16, kWavesMany = 4;
+// Weight tiles of a workgroup, which share its activations: 4 where enough workgroups are left (7 rows through
+// 151936 x 4096 60 us, 67 with 2; 32 rows through 24576 x 4096 17.8, 18.8). One row asks for more of them: through
+// 24576 x 4096 12.9, with 2 tiles 12.2.
+constexpr uint32_t kQuadFrom = 1024, kQuadFromWide = 256, kPairFrom = 256;
+
+__device__ __forceinline__ bf16x8 unpack_w4(uint32_t w, uint32_t mask, uint32_t base) {
+  // Eight nibbles to bf16 16 + q.
+  const u32x4 v = {((w << 3) & mask) | base, ((w >> 1) & mask) | base, ((w >> 5) & mask) | base,
+                   ((w >> 9) & mask) | base};
   return __builtin_bit_cast(bf16x8, v);
 }
 
 // One workgroup: NT consecutive 16-row weight tiles and one split of k, whose
 // 128-column blocks its waves divide; wave partials are added in wave order
 // through LDS. GB: 32-column k-blocks per group. MT: 16-row activation tiles.
+// A wave has one block in flight and leaves the rest to the other waves of its SIMD, up to 8:
+// with two or three in flight, which take the registers of as many waves, nothing was
+// faster (32 rows through 24576 x 4096: 20.3 us with two, 17.8 with one).
 template <int NT, int MT, int GB, bool ZP, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void gemm_w4_kernel(const uint16_t* __restrict__ xt,
-                                                            const uint32_t* __restrict__ w,
-                                                            const uint16_t* __restrict__ scales,
-                                                            const uint8_t* __restrict__ zeros, uint32_t m,
-                                                            uint32_t kb_count, uint32_t kb_split, uint32_t epi,
-                                                            const uint16_t* residual, void* out, uint32_t ldo,
-                                                            uint32_t* err) {
+__global__ __launch_bounds__(WAVES * 64, WAVES == 4 && (NT == 4 || MT == 2) ? 3 : 4) void gemm_w4_kernel(
+    const uint16_t* __restrict__ xt, const uint32_t* __restrict__ w, const uint16_t* __restrict__ scales,
+    const uint8_t* __restrict__ zeros, uint32_t m, uint32_t kb_count, uint32_t kb_split, uint32_t epi,
+    const uint16_t* residual, void* out, uint32_t ldo, uint32_t* err) {
   constexpr int GP = 4 / GB;  // groups per 128 columns
   __shared__ float red[WAVES][NT * MT * 256];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -59,92 +77,123 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_w4_kernel(const uint16_t* __r
   const uint32_t kb_lo = s_lo + (s_n * wave) / WAVES, kb_hi = s_lo + (s_n * (wave + 1)) / WAVES;
   const uint32_t r16 = lane & 15, g16 = lane >> 4;
 
-  struct Stage {
+  struct Block {
     u32x4 w[NT], x[4][MT];
-    uint2 s[NT][GP];
-    uint32_t z[ZP ? NT : 1][GP];
+    uint32_t s[NT];           // scale of row lane % 16, group lane / 16 % GP
+    uint32_t z[ZP ? NT : 1];  // its zero point
   };
-  const uint64_t kg = (uint64_t)kb_count * GP;
-  auto load = [&](Stage& st, uint32_t kb) {
+  // Buffers: uniform bases, one 32-bit offset a lane.
+  const uint32_t wbytes = kb_count * 1024, sbytes = kb_count * 32 * GP, zbytes = kb_count * 16 * GP;
+  auto buffer = [](const void* p, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, bytes, 0x00020000);
+  };
+  const auto wr = buffer(reinterpret_cast<const char*>(w) + (uint64_t)tile0 * wbytes, NT * wbytes);
+  const auto sr = buffer(reinterpret_cast<const char*>(scales) + (uint64_t)tile0 * sbytes, NT * sbytes);
+  const auto zr = buffer(reinterpret_cast<const char*>(zeros) + (uint64_t)tile0 * zbytes, NT * zbytes);
+  const auto xr = buffer(xt, kb_count * 8192);
+  uint32_t xoff[MT];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      st.w[nt] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(w) +
-                                            ((uint64_t)(tile0 + nt) * kb_count + kb) * 64 + lane);
-#pragma unroll
-      for (int p = 0; p < GP; ++p) {
-        const uint64_t at = ((uint64_t)(tile0 + nt) * kg + kb * GP + p) * 16 + 4 * g16;
-        st.s[nt][p] = *reinterpret_cast<const uint2*>(scales + at);
-        if constexpr (ZP) st.z[nt][p] = *reinterpret_cast<const uint32_t*>(zeros + at);
-      }
-    }
+  for (int mt = 0; mt < MT; ++mt) xoff[mt] = mt * 1024 + (min(16 * mt + r16, m - 1) & 15u) * 16 + g16 * 256;
+  auto load = [&](Block& b, uint32_t kb) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        const uint32_t row = min(16 * mt + r16, m - 1) & 15u;
-        st.x[j][mt] = *(reinterpret_cast<const u32x4*>(xt) + ((uint64_t)(4 * kb + j) * 2 + mt) * 64 + row + 16 * g16);
-      }
+      for (int mt = 0; mt < MT; ++mt)
+        b.x[j][mt] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                    xr, xoff[mt] + (j & 1) * 2048, kb * 8192 + (j >> 1) * 4096, 0));
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      b.w[nt] = __builtin_bit_cast(
+          u32x4, __builtin_amdgcn_raw_buffer_load_b128(wr, lane * 16, nt * wbytes + kb * 1024, 2));  // non-temporal
+      const uint32_t sat = nt * sbytes + kb * 32 * GP;
+      const uint32_t at = g16 % GP * 16 + r16;
+      b.s[nt] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(sr, at * 2, sat, 0);
+      if constexpr (ZP) b.z[nt] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(zr, at, nt * zbytes + kb * 16 * GP, 0);
+    }
   };
+  // In registers, so that a mask and an or are one instruction.
+  uint32_t mask = 0x00780078u, base = 0x41804180u;
+  asm volatile("" : "+s"(mask));
+  asm volatile("" : "+v"(base));
 
   f32x4 acc[NT][MT];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) acc[nt][mt] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const bf16x8 ones = __builtin_bit_cast(bf16x8, u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
-  auto compute = [&](const Stage& st) {
+  // bf16 -16 (with zero points) or -24.
+  constexpr uint32_t kOff = ZP ? 0xc180c180u : 0xc1c0c1c0u;
+  const bf16x8 offset = __builtin_bit_cast(bf16x8, u32x4{kOff, kOff, kOff, kOff});
+  auto compute = [&](const Block& b) {
+    // Scale (low half) and zero point of a group in all lanes of its row: the lanes' words, their 16-lane groups
+    // exchanged.
+    uint32_t sz[NT][GP];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      uint32_t v = b.s[nt];
+      if constexpr (ZP) v |= b.z[nt] << 16;
+      if constexpr (GP == 1) {
+        sz[nt][0] = v;
+      } else if constexpr (GP == 2) {
+        const auto t = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        sz[nt][0] = t[0];
+        sz[nt][1] = t[1];
+      } else {
+        const auto u = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        const auto t0 = __builtin_amdgcn_permlane16_swap(u[0], u[0], false, false);
+        const auto t1 = __builtin_amdgcn_permlane16_swap(u[1], u[1], false, false);
+        sz[nt][0] = t0[0];
+        sz[nt][1] = t0[1];
+        sz[nt][2] = t1[0];
+        sz[nt][3] = t1[1];
+      }
+    }
 #pragma unroll
     for (int p = 0; p < GP; ++p) {
-      f32x4 sx[MT], part[NT][MT];
+      f32x4 part[NT][MT], sx[MT];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         sx[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
+        for (int i = 0; i < GB; ++i)
+          sx[mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b.x[p * GB + i][mt]), offset,
+                                                           sx[mt], 0, 0, 0);
+#pragma unroll
         for (int nt = 0; nt < NT; ++nt) part[nt][mt] = sx[mt];
       }
 #pragma unroll
-      for (int b = 0; b < GB; ++b) {
-        const int j = p * GB + b;
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-          sx[mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, __builtin_bit_cast(bf16x8, st.x[j][mt]), sx[mt], 0, 0, 0);
+      for (int i = 0; i < GB; ++i) {
+        const int j = p * GB + i;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          const bf16x8 a = unpack_w4(st.w[nt][j]);
+          const bf16x8 q = unpack_w4(b.w[nt][j], mask, base);
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt)
-            part[nt][mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, __builtin_bit_cast(bf16x8, st.x[j][mt]),
+            part[nt][mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b.x[j][mt]), q,
                                                                   part[nt][mt], 0, 0, 0);
         }
       }
-      // Lane: activation row r16, weight rows 4 g16 + e.
+      // Lane: weight row r16, activation rows 4 g16 + e.
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const float s[4] = {lo_bf16(st.s[nt][p].x), hi_bf16(st.s[nt][p].x), lo_bf16(st.s[nt][p].y),
-                            hi_bf16(st.s[nt][p].y)};
+        const float s = lo_bf16(sz[nt][p]);
+        // sx is -16 times the activations' sum.
+        const float z = ZP ? 0.0625f * (float)((sz[nt][p] >> 16) & 0xffu) : 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float z = ZP ? 128.f + (float)((st.z[ZP ? nt : 0][p] >> (8 * e)) & 0xffu) : 136.f;
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
-            acc[nt][mt][e] = __builtin_fmaf(s[e], __builtin_fmaf(-z, sx[mt][e], part[nt][mt][e]), acc[nt][mt][e]);
-        }
+          for (int e = 0; e < 4; ++e) {
+            const float v = ZP ? __builtin_fmaf(z, sx[mt][e], part[nt][mt][e]) : part[nt][mt][e];
+            acc[nt][mt][e] = __builtin_fmaf(s, v, acc[nt][mt][e]);
+          }
       }
     }
   };
-  Stage a, b;
-  if (kb_lo < kb_hi) load(a, kb_lo);
-  for (uint32_t kb = kb_lo; kb < kb_hi; kb += 2) {
-    if (kb + 1 < kb_hi) load(b, kb + 1);
-    __builtin_amdgcn_sched_barrier(0);
-    compute(a);
-    __builtin_amdgcn_sched_barrier(0);
-    if (kb + 1 < kb_hi) {
-      if (kb + 2 < kb_hi) load(a, kb + 2);
-      __builtin_amdgcn_sched_barrier(0);
-      compute(b);
-      __builtin_amdgcn_sched_barrier(0);
-    }
+  for (uint32_t kb = kb_lo; kb < kb_hi; ++kb) {
+    Block b;
+    load(b, kb);
+    __builtin_amdgcn_sched_barrier(0);  // all of the block's loads are on their way before the first wait
+    compute(b);
   }
 
 #pragma unroll
@@ -152,7 +201,7 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_w4_kernel(const uint16_t* __r
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) red[wave][(nt * MT + mt) * 256 + r16 * 16 + 4 * g16 + e] = acc[nt][mt][e];
+      for (int e = 0; e < 4; ++e) red[wave][(nt * MT + mt) * 256 + (4 * g16 + e) * 16 + r16] = acc[nt][mt][e];
   __syncthreads();
   auto total = [&](int i) {
     float v = red[0][i];
@@ -263,8 +312,8 @@ void launch_w4_kernel(const uint16_t* xt, const uint32_t* w, const uint16_t* sca
                       uint32_t n, uint32_t k, uint32_t epi, uint32_t splits, const uint16_t* residual, void* out,
                       uint32_t ldo, uint32_t* err, hipStream_t s) {
   const uint32_t kb = k / 128;
-  hipLaunchKernelGGL((gemm_w4_kernel<NT, MT, GB, ZP, WAVES>), dim3(n / (16 * NT), splits), dim3(WAVES * 64), 0, s, xt, w,
-                     scales, zeros, m, kb, (kb + splits - 1) / splits, epi, residual, out, ldo, err);
+  hipLaunchKernelGGL((gemm_w4_kernel<NT, MT, GB, ZP, WAVES>), dim3(n / (16 * NT), splits), dim3(WAVES * 64), 0, s, xt,
+                     w, scales, zeros, m, kb, (kb + splits - 1) / splits, epi, residual, out, ldo, err);
 }
 
 template <int NT, int WAVES>
@@ -297,11 +346,23 @@ hipError_t launch_gemm_w4(const uint16_t* x_tiled, const uint32_t* w_tiled, cons
                           const uint8_t* zeros, uint32_t m, uint32_t n, uint32_t k, uint32_t group, uint32_t epilogue,
                           uint32_t splits, const uint16_t* residual, void* out, uint32_t ldo, uint32_t* err,
                           hipStream_t s) {
-  const bool pair = n % 32 == 0 && (epilogue == FH_EPI_SWIGLU || n / 32 * splits >= 256);
-  if (pair)
-    launch_w4<2, 8>(x_tiled, w_tiled, scales, zeros, m, n, k, group, epilogue, splits, residual, out, ldo, err, s);
+  const uint64_t wide = (uint64_t)splits * n;
+  const bool quad = n % 64 == 0 && wide / 64 >= (m > 8 ? kQuadFromWide : kQuadFrom);
+  const bool pair = n % 32 == 0 && (epilogue == FH_EPI_SWIGLU || wide / 32 >= kPairFrom);
+  const bool many = wide / (pair ? 32 : 16) >= kMany;
+#define FH_NT(NT_, WAVES_)                                                                                          \
+  launch_w4<NT_, WAVES_>(x_tiled, w_tiled, scales, zeros, m, n, k, group, epilogue, splits, residual, out, ldo, err, s)
+  if (quad)
+    FH_NT(4, kWavesMany);
+  else if (pair && many)
+    FH_NT(2, kWavesMany);
+  else if (pair)
+    FH_NT(2, kWavesFew);
+  else if (many)
+    FH_NT(1, kWavesMany);
   else
-    launch_w4<1, 8>(x_tiled, w_tiled, scales, zeros, m, n, k, group, epilogue, splits, residual, out, ldo, err, s);
+    FH_NT(1, kWavesFew);
+#undef FH_NT
   return hipGetLastError();
 }
 

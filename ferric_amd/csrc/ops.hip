@@ -35,7 +35,7 @@ inline bool prefix_shape_ok(uint32_t rows, uint32_t qh, uint32_t kvh, uint32_t c
 }
 
 inline bool w4_shape_ok(uint32_t n, uint32_t k, uint32_t group) {
-  return n != 0 && k != 0 && n % 16 == 0 && k % 128 == 0 && (group == 32 || group == 64 || group == 128);
+  return n != 0 && k != 0 && n % 16 == 0 && k % 128 == 0 && k <= 1u << 24 && (group == 32 || group == 64 || group == 128);
 }
 
 #define from_hip(expr) (static_cast<void>(hipGetLastError()), status_of(expr))

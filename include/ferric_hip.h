@@ -272,8 +272,8 @@ fh_status fh_op_gemm(const uint16_t* x_tiled, const uint16_t* w_tiled, uint32_t 
 /* K1 projections with 4-bit weights and group scales, for decode batches (1 <= m <= 32):
  * out = epilogue(x[m][k] . W[n][k]^T), W[n][k] = scale[n][k / group] * (q[n][k] - zero[n][k / group]),
  * q in 0..15, zero 8 where zeros_tiled is NULL; FP32 accumulation on MFMA (the quantized
- * weights enter it exactly). n % 16 == 0 (32 for FH_EPI_SWIGLU), k % 128 == 0, group 32, 64
- * or 128. Epilogues, x_tiled, splits (<= k / 128 and 65535), residual, out, ldo and error_word as
+ * weights enter it exactly). n % 16 == 0 (32 for FH_EPI_SWIGLU), k % 128 == 0, k <= 2^24, group
+ * 32, 64 or 128. Epilogues, x_tiled, splits (<= k / 128 and 65535), residual, out, ldo and error_word as
  * fh_op_gemm; only the first m rows of out are written. Operands in the order
  * fh_op_tile_weight_w4 writes, w_tiled and x_tiled 16-byte, scales_tiled 8-byte and
  * zeros_tiled 4-byte aligned. No counterpart in the reference, whose projections read bf16

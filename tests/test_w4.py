@@ -15,7 +15,7 @@ def gemm(x=P, w=P, s=P, z=None, m=1, n=32, k=256, group=64, epi=0, splits=1, res
     return LIB.fh_op_gemm_w4(x, w, s, z, m, n, k, group, epi, splits, residual, out, ldo, None, None)
 
 
-@pytest.mark.parametrize("bad", [dict(x=None), dict(w=None), dict(s=None), dict(out=None), dict(m=0), dict(m=33), dict(n=0),
+@pytest.mark.parametrize("bad", [dict(x=None), dict(w=None), dict(s=None), dict(out=None), dict(m=0), dict(m=33), dict(k=(1 << 24) + 128), dict(n=0),
                                  dict(n=24), dict(k=0), dict(k=192), dict(group=16), dict(group=256), dict(group=0),
                                  dict(epi=5), dict(splits=0), dict(splits=2), dict(epi=4, splits=3), dict(epi=1), dict(ldo=31),
                                  dict(epi=2, n=16), dict(x=P + 8), dict(w=P + 8), dict(s=P + 4), dict(z=P + 2),
