@@ -119,11 +119,13 @@ SIGNATURES = [
     ("fh_read_kv_cache", _st, [_vp, _u32, _u32, _u16p, _u64]),
     ("fh_kv_copy_pages", _st, [_vp, _vp, _u32]),
     ("fh_execute_batch", _st, [_vp, _u64, ctypes.POINTER(Row), _u32, _u32p, _u32, _u32p]),
+    ("fh_execute_batch_shared", _st, [_vp, _u64, ctypes.POINTER(Row), _u32, _vp, _u32, _u32p, _u32, _u32p]),
     ("fh_read_logits", _st, [_vp, _f32p, _u64]),
     ("fh_read_hidden", _st, [_vp, _u32, _u16p, _u64]),
     ("fh_row_capacity", _u32, [_vp]),
     ("fh_dispatch_count", _u64, [_vp]),
     ("fh_expected_dispatch_count", _st, [_vp, _u64, ctypes.POINTER(Row), _u32, _u32p, _u32, _u64p]),
+    ("fh_expected_dispatch_count_shared", _st, [_vp, _u64, ctypes.POINTER(Row), _u32, _vp, _u32, _u32p, _u32, _u64p]),
     ("fh_last_step_ms", ctypes.c_float, [_vp]),
     ("fh_set_profiling", _st, [_vp, _u32]),
     ("fh_kernel_class_ms", _st, [_vp, _u32, _f32p, _u32p]),

@@ -149,6 +149,26 @@ struct fh_ctx {
   };
   std::map<uint32_t, StepGraph> graphs;
   std::vector<hipGraph_t> graph_defs;
+
+  // Decode steps whose rows share prefixes (fh_execute_batch_shared): the groups of the last
+  // step (none: every row for itself) and the scratch their attention needs, grown on demand. A
+  // step with the rows and groups of the shared step before it is captured and then replayed;
+  // the graph of other ones is dropped, so their number is one.
+  std::vector<fh_prefix_group> last_groups;
+  void* prefix_scratch = nullptr;
+  uint64_t prefix_scratch_size = 0;
+  struct SharedGraph {
+    uint32_t rows = 0;
+    std::vector<fh_prefix_group> groups;
+    hipGraph_t def = nullptr;
+    StepGraph step;
+    void drop() {
+      if (step.exec) hipGraphExecDestroy(step.exec);
+      if (def) hipGraphDestroy(def);
+      step = StepGraph{};
+      def = nullptr;
+    }
+  } shared;
   hipEvent_t ev_begin = nullptr, ev_end = nullptr;
   float last_ms = 0.f;
 
@@ -465,8 +485,21 @@ fh::AttnQkn step_qkn_args(fh_ctx* ctx, uint32_t l) {
                      kv_cache(ctx, l, 1), ctx->md.rms_epsilon};
 }
 
-// Enqueues (or, dry, only counts) the launches of a decode step of R rows.
-hipError_t enqueue_step(fh_ctx* ctx, uint32_t R, uint64_t* launches, bool dry = false) {
+using PrefixGroups = std::vector<fh_prefix_group>;
+
+hipError_t launch_shared_attention(fh_ctx* ctx, uint32_t l, uint32_t R, const PrefixGroups& groups) {
+  const fh_ctx_options& op = ctx->opt;
+  const uint32_t* d_pos = ctx->d_meta + op.row_capacity;
+  return fh::launch_prefix_attention(ctx->qrot, kv_cache(ctx, l, 0), kv_cache(ctx, l, 1), d_pos,
+                                     d_pos + op.row_capacity, groups.data(), (uint32_t)groups.size(), ctx->attn, 1,
+                                     ctx->prefix_scratch, R, ctx->md.query_heads, ctx->md.kv_heads,
+                                     op.page_table_stride, op.physical_pages, op.context_tokens, ctx->err,
+                                     ctx->stream);
+}
+
+// Enqueues (or, dry, only counts) the launches of a decode step of R rows, which share the prefixes of `groups`
+// (none: the attention of every row for itself).
+hipError_t enqueue_step(fh_ctx* ctx, uint32_t R, const PrefixGroups& groups, uint64_t* launches, bool dry = false) {
   const fh_model_desc& md = ctx->md;
   const fh_ctx_options& op = ctx->opt;
   hipStream_t s = ctx->stream;
@@ -491,7 +524,7 @@ hipError_t enqueue_step(fh_ctx* ctx, uint32_t R, uint64_t* launches, bool dry = 
   const uint32_t sq = ctx->s_qkv, so = ctx->s_o, sd = ctx->s_down;
   const uint32_t split = fh::attn_split_pages(R, QH, KVH, C);
   const bool fuse = fh::attn_fuse_merge(R, KVH, C, split);
-  const bool qkn = step_runs_qkn(ctx, R);
+  const bool qkn = groups.empty() && step_runs_qkn(ctx, R);
   // The step's tokens, positions and page tables come in from the pinned
   // host mirror by the first launch, so a replayed graph needs no copy beside it.
   const uint32_t meta_words = 2 * cap + R * stride;
@@ -548,16 +581,21 @@ hipError_t enqueue_step(fh_ctx* ctx, uint32_t R, uint64_t* launches, bool dry = 
                                          d_pos, d_tab, ctx->qrot, kc, vc, R, QH, KVH, stride, P, C, md.rms_epsilon,
                                          err, s);
       });
-    const fh::AttnQkn qa = step_qkn_args(ctx, l);
-    L(FH_KC_ATTENTION, [&] {
-      return fh::launch_attention_partial(ctx->qrot, kc, vc, d_pos, d_tab, ctx->attn_part, ctx->attn, 1, 0, R, R, QH,
-                                          KVH, stride, P, C, split, fuse ? ctx->attn_count : nullptr, err, s,
-                                          qkn ? &qa : nullptr);
-    });
-    if (!fuse)
-      L(FH_KC_ATTENTION_MERGE, [&] {
-        return fh::launch_attention_merge(ctx->attn_part, d_pos, ctx->attn, 1, 0, R, R, QH, C, split, err, s);
+    if (!groups.empty()) {
+      L(FH_KC_ATTENTION, [&] { return launch_shared_attention(ctx, l, R, groups); });
+      ++n;  // prefixes, then own keys and the merge: two launches
+    } else {
+      const fh::AttnQkn qa = step_qkn_args(ctx, l);
+      L(FH_KC_ATTENTION, [&] {
+        return fh::launch_attention_partial(ctx->qrot, kc, vc, d_pos, d_tab, ctx->attn_part, ctx->attn, 1, 0, R, R, QH,
+                                            KVH, stride, P, C, split, fuse ? ctx->attn_count : nullptr, err, s,
+                                            qkn ? &qa : nullptr);
       });
+      if (!fuse)
+        L(FH_KC_ATTENTION_MERGE, [&] {
+          return fh::launch_attention_merge(ctx->attn_part, d_pos, ctx->attn, 1, 0, R, R, QH, C, split, err, s);
+        });
+    }
     L(FH_KC_O_GEMM, [&] {
       return fh::launch_gemm(ctx->attn, W.o, R, H, Q, FH_EPI_PARTIAL, so, nullptr, ctx->o_part, H, err, s);
     });
@@ -820,6 +858,8 @@ void fh_destroy(fh_ctx* ctx) {
   if (ctx->stream) hipStreamSynchronize(ctx->stream);
   for (auto& kv : ctx->graphs) hipGraphExecDestroy(kv.second.exec);
   for (auto g : ctx->graph_defs) hipGraphDestroy(g);
+  ctx->shared.drop();
+  if (ctx->prefix_scratch) hipFree(ctx->prefix_scratch);
   for (auto ev : ctx->prof_events) hipEventDestroy(ev);
   if (ctx->ev_begin) hipEventDestroy(ctx->ev_begin);
   if (ctx->ev_end) hipEventDestroy(ctx->ev_end);
@@ -1321,14 +1361,57 @@ void await_choices(const uint32_t* done, uint32_t rows) {
     }
 }
 
-fh_status fh_execute_batch(fh_ctx* ctx, uint64_t batch_id, const fh_row* rows, uint32_t nrows,
-                           const uint32_t* output_rows, uint32_t nout, uint32_t* choices_out) {
-  if (!ctx) return FH_ERR_INVALID_ARGUMENT;
-  if (nout && (!output_rows || !choices_out)) return fail(ctx, FH_ERR_INVALID_ARGUMENT, "null output buffers");
-  fh_status st = validate_batch(ctx, batch_id, rows, nrows, output_rows, nout);
-  if (st != FH_OK) return st;
-  if (nrows > ctx->opt.row_capacity) return run_prefill(ctx, batch_id, rows, nrows, output_rows, nout, choices_out);
+// Why the groups of a validated decode batch are refused, or nullptr: every row of a group has to list the
+// prefix's pages at the start of its list and to write behind them.
+const char* shared_rows_refused(const fh_ctx* ctx, const fh_row* rows, uint32_t nrows, const fh_prefix_group* groups,
+                                uint32_t ngroups) {
+  if (nrows > ctx->opt.row_capacity) return "prefix groups: decode batches only";
+  if (const char* why = fh::prefix_groups_refused(groups, ngroups, nrows, ctx->opt.context_tokens)) return why;
+  for (uint32_t i = 0; i < ngroups; ++i) {
+    const fh_prefix_group& g = groups[i];
+    if (g.prefix_pages == 0) return "prefix groups: a prefix without pages";
+    const fh_row& first = rows[g.first_row];
+    for (uint32_t j = 0; j < g.rows; ++j) {
+      const fh_row& r = rows[g.first_row + j];
+      if (r.position / kPageTokens < g.prefix_pages) return "prefix groups: a row writes into its prefix";
+      if (std::memcmp(r.pages, first.pages, g.prefix_pages * 4ull) != 0)
+        return "prefix groups: the rows' page lists differ within the prefix";
+    }
+  }
+  return nullptr;
+}
 
+fh_status run_step(fh_ctx* ctx, uint64_t batch_id, const fh_row* rows, uint32_t nrows, const PrefixGroups& groups,
+                   const uint32_t* output_rows, uint32_t nout, uint32_t* choices_out) {
+  auto same = [](const PrefixGroups& a, const PrefixGroups& b) {
+    return a.size() == b.size() && (a.empty() || std::memcmp(a.data(), b.data(), a.size() * sizeof(a[0])) == 0);
+  };
+  // (The stream is idle here: every step ends with a synchronize.)
+  const bool shared_again = !groups.empty() && ctx->shared.rows == nrows && same(ctx->shared.groups, groups);
+  if (!groups.empty() && !shared_again) {
+    ctx->shared.drop();
+    ctx->shared.rows = 0;
+    const uint64_t need = fh::prefix_scratch_bytes(groups.data(), (uint32_t)groups.size(), nrows, ctx->md.query_heads,
+                                                   ctx->md.kv_heads);
+    if (need > ctx->prefix_scratch_size) {
+      // The old one stays until there is a new one: fh_time_attention may still use it.
+      int device = -1;
+      void* scratch = nullptr;
+      hipError_t me = hipGetDevice(&device);
+      if (me == hipSuccess) me = hipSetDevice(ctx->opt.device);
+      if (me == hipSuccess) me = hipMalloc(&scratch, need);
+      if (device >= 0) (void)hipSetDevice(device);
+      if (me != hipSuccess) {
+        (void)hipGetLastError();
+        return fail(ctx, FH_ERR_OUT_OF_MEMORY, "hipMalloc of " + std::to_string(need) + " bytes failed");
+      }
+      if (ctx->prefix_scratch) hipFree(ctx->prefix_scratch);
+      ctx->prefix_scratch = scratch;
+      ctx->prefix_scratch_size = need;
+    }
+    ctx->shared.groups = groups;
+    ctx->shared.rows = nrows;
+  }
   const uint32_t cap = ctx->opt.row_capacity, stride = ctx->opt.page_table_stride;
   uint32_t* tok = ctx->h_meta;
   uint32_t* pos = ctx->h_meta + cap;
@@ -1351,31 +1434,45 @@ fh_status fh_execute_batch(fh_ctx* ctx, uint64_t batch_id, const fh_row* rows, u
   hipEventRecord(ctx->ev_begin, s);
   uint64_t launches = 0;
   if (ctx->profiling) ctx->prof_launches.clear();
-  if (ctx->opt.use_graphs && !ctx->profiling) {
+  const bool graphs = ctx->opt.use_graphs && !ctx->profiling;
+  auto capture = [&](hipGraph_t* g, hipGraphExec_t* ge) {
+    e = hipStreamBeginCapture(s, hipStreamCaptureModeThreadLocal);
+    if (e == hipSuccess) {
+      hipError_t le = enqueue_step(ctx, nrows, groups, &launches);
+      e = hipStreamEndCapture(s, g);
+      if (e == hipSuccess && le != hipSuccess) e = le;
+    }
+    if (e == hipSuccess) e = hipGraphInstantiate(ge, *g, nullptr, nullptr, 0);
+    if (e == hipSuccess) return FH_OK;
+    if (*g) hipGraphDestroy(*g);
+    *g = nullptr;
+    return poison(FH_ERR_DEVICE, std::string("graph capture: ") + hipGetErrorString(e));
+  };
+  if (graphs && shared_again) {
+    fh_ctx::SharedGraph& sg = ctx->shared;
+    if (!sg.step.exec) {
+      const fh_status st = capture(&sg.def, &sg.step.exec);
+      if (st != FH_OK) return st;
+      sg.step.launches = launches;
+    }
+    launches = sg.step.launches;
+    e = hipGraphLaunch(sg.step.exec, s);
+  } else if (graphs && groups.empty()) {
     // One graph per row count and per form of the attention stage.
     const uint32_t key = nrows | (step_runs_qkn(ctx, nrows) ? 1u << 16 : 0u);
     auto it = ctx->graphs.find(key);
     if (it == ctx->graphs.end()) {
       hipGraph_t g = nullptr;
       hipGraphExec_t ge = nullptr;
-      e = hipStreamBeginCapture(s, hipStreamCaptureModeThreadLocal);
-      if (e == hipSuccess) {
-        hipError_t le = enqueue_step(ctx, nrows, &launches);
-        e = hipStreamEndCapture(s, &g);
-        if (e == hipSuccess && le != hipSuccess) e = le;
-      }
-      if (e == hipSuccess) e = hipGraphInstantiate(&ge, g, nullptr, nullptr, 0);
-      if (e != hipSuccess) {
-        if (g) hipGraphDestroy(g);
-        return poison(FH_ERR_DEVICE, std::string("graph capture: ") + hipGetErrorString(e));
-      }
+      const fh_status st = capture(&g, &ge);
+      if (st != FH_OK) return st;
       ctx->graph_defs.push_back(g);
       it = ctx->graphs.emplace(key, fh_ctx::StepGraph{ge, launches}).first;
     }
     launches = it->second.launches;  // a replay issues what its capture recorded
     e = hipGraphLaunch(it->second.exec, s);
   } else {
-    e = enqueue_step(ctx, nrows, &launches);
+    e = enqueue_step(ctx, nrows, groups, &launches);
   }
   if (e != hipSuccess) return poison(FH_ERR_DEVICE, std::string("launch: ") + hipGetErrorString(e) + ctx->launch_detail);
   hipEventRecord(ctx->ev_end, s);
@@ -1387,7 +1484,8 @@ fh_status fh_execute_batch(fh_ctx* ctx, uint64_t batch_id, const fh_row* rows, u
   if (ctx->profiling) collect_profile(ctx);
   ctx->last_rows = nrows;
   ctx->last_batch_rows = nrows;
-  ctx->last_qkn = step_runs_qkn(ctx, nrows);
+  ctx->last_qkn = groups.empty() && step_runs_qkn(ctx, nrows);
+  ctx->last_groups = groups;
   ctx->last_logits = ctx->logits;
   ctx->last_was_prefill = false;
   const uint32_t errw = ctx->h_out[cap];
@@ -1400,6 +1498,29 @@ fh_status fh_execute_batch(fh_ctx* ctx, uint64_t batch_id, const fh_row* rows, u
   ctx->last_batch = batch_id;
   ctx->dispatches += launches;
   return FH_OK;
+}
+
+fh_status fh_execute_batch(fh_ctx* ctx, uint64_t batch_id, const fh_row* rows, uint32_t nrows,
+                           const uint32_t* output_rows, uint32_t nout, uint32_t* choices_out) {
+  if (!ctx) return FH_ERR_INVALID_ARGUMENT;
+  if (nout && (!output_rows || !choices_out)) return fail(ctx, FH_ERR_INVALID_ARGUMENT, "null output buffers");
+  fh_status st = validate_batch(ctx, batch_id, rows, nrows, output_rows, nout);
+  if (st != FH_OK) return st;
+  if (nrows > ctx->opt.row_capacity) return run_prefill(ctx, batch_id, rows, nrows, output_rows, nout, choices_out);
+  return run_step(ctx, batch_id, rows, nrows, {}, output_rows, nout, choices_out);
+}
+
+fh_status fh_execute_batch_shared(fh_ctx* ctx, uint64_t batch_id, const fh_row* rows, uint32_t nrows,
+                                  const fh_prefix_group* groups, uint32_t ngroups, const uint32_t* output_rows,
+                                  uint32_t nout, uint32_t* choices_out) {
+  if (ngroups == 0) return fh_execute_batch(ctx, batch_id, rows, nrows, output_rows, nout, choices_out);
+  if (!ctx) return FH_ERR_INVALID_ARGUMENT;
+  if (nout && (!output_rows || !choices_out)) return fail(ctx, FH_ERR_INVALID_ARGUMENT, "null output buffers");
+  fh_status st = validate_batch(ctx, batch_id, rows, nrows, output_rows, nout);
+  if (st != FH_OK) return st;
+  if (const char* why = shared_rows_refused(ctx, rows, nrows, groups, ngroups))
+    return fail(ctx, FH_ERR_INVALID_ARGUMENT, why);
+  return run_step(ctx, batch_id, rows, nrows, PrefixGroups(groups, groups + ngroups), output_rows, nout, choices_out);
 }
 
 fh_status fh_read_logits(fh_ctx* ctx, float* out, uint64_t elements) {
@@ -1436,7 +1557,23 @@ fh_status fh_expected_dispatch_count(fh_ctx* ctx, uint64_t batch_id, const fh_ro
     enqueue_prefill(ctx, nrows, nout, nblocks, form, 0, priv, &n, true);
   }
   else
-    enqueue_step(ctx, nrows, &n, true);
+    enqueue_step(ctx, nrows, {}, &n, true);
+  *count = n;
+  return FH_OK;
+}
+
+fh_status fh_expected_dispatch_count_shared(fh_ctx* ctx, uint64_t batch_id, const fh_row* rows, uint32_t nrows,
+                                            const fh_prefix_group* groups, uint32_t ngroups,
+                                            const uint32_t* output_rows, uint32_t nout, uint64_t* count) {
+  if (ngroups == 0) return fh_expected_dispatch_count(ctx, batch_id, rows, nrows, output_rows, nout, count);
+  if (!ctx || !count) return FH_ERR_INVALID_ARGUMENT;
+  if (nout && !output_rows) return fail(ctx, FH_ERR_INVALID_ARGUMENT, "null output rows");
+  fh_status st = validate_batch(ctx, batch_id, rows, nrows, output_rows, nout);
+  if (st != FH_OK) return st;
+  if (const char* why = shared_rows_refused(ctx, rows, nrows, groups, ngroups))
+    return fail(ctx, FH_ERR_INVALID_ARGUMENT, why);
+  uint64_t n = 0;
+  enqueue_step(ctx, nrows, PrefixGroups(groups, groups + ngroups), &n, true);
   *count = n;
   return FH_OK;
 }
@@ -1470,6 +1607,7 @@ fh_status fh_time_attention(fh_ctx* ctx, uint32_t reps, float* avg_ms) {
   const uint32_t* d_tab = ctx->d_meta + 2 * cap;
   hipStream_t s = ctx->stream;
   auto launch = [&] {
+    if (!ctx->last_groups.empty()) return launch_shared_attention(ctx, l, R, ctx->last_groups);
     const uint32_t split = fh::attn_split_pages(R, md.query_heads, md.kv_heads, op.context_tokens);
     const bool fuse = fh::attn_fuse_merge(R, md.kv_heads, op.context_tokens, split);
     // The attention kernel class of the step: the partition launch (with the

@@ -17,6 +17,8 @@ import numpy as np
 
 from .runner import PAGE_TOKENS, PagedLimits, PreparedBatch, PreparedRow, PreparedRows
 
+MAX_PREFIX_GROUPS = 64  # of one call (fh_op_prefix_attention)
+
 
 class SequenceState:
     """A sequence's committed length and its logical-to-physical page list,
@@ -308,6 +310,33 @@ class PagePool:
             self._shared[int(p)] = self._shared.get(int(p), 1) + 1
         self.sequences[new.sequence] = new
         return new.sequence, moves
+
+    @staticmethod
+    def prefix_groups(batch: PreparedBatch, min_pages: int = 1) -> list:
+        """Runs of consecutive rows of a decode batch that list the same pages
+        first, as TpBatchRunner.execute_batch takes them: [(first row, rows, prefix
+        pages)]. Only whole pages before every row's written one count. A run goes
+        on while the page reads saved, (rows - 1) * pages, do not fall. Sharing
+        gains from about 8 rows on at any length (device time of a step, Qwen3-8B
+        shape, one prompt: 32 rows behind 8192 tokens 11.39 -> 4.25 ms, behind 64
+        4.22 -> 3.80), with fewer rows from about 1000 tokens (4 rows: 3.58 -> 3.46
+        ms; behind 64 tokens 3.37 -> 3.43); min_pages leaves shorter ones out."""
+        lists = [(np.asarray(r.physical_pages), r.position // PAGE_TOKENS) for r in batch.rows]
+        groups, i = [], 0
+        while i < len(lists):
+            pages, n, rows = lists[i][0], lists[i][1], 1
+            while i + rows < len(lists):
+                other, most = lists[i + rows]
+                most = min(n, most, len(other))
+                differ = np.flatnonzero(pages[:most] != other[:most])
+                m = int(differ[0]) if len(differ) else most
+                if m < min_pages or rows * m < (rows - 1) * n:
+                    break
+                n, rows = m, rows + 1
+            if rows > 1:
+                groups.append((i, rows, n))
+            i += rows
+        return groups[:MAX_PREFIX_GROUPS]
 
     def compact(self) -> list:
         """Moves the pages in use to the lowest page ids and returns the moves

@@ -210,6 +210,16 @@ def _page_array(pages) -> np.ndarray:
     return np.ascontiguousarray(np.asarray(pages, dtype=np.uint32))
 
 
+def _groups_to_c(groups) -> np.ndarray:
+    """fh_prefix_group[] as a uint32 array [groups][3]."""
+    g = np.asarray(groups)
+    if g.size == 0:
+        return np.zeros((0, 3), dtype=np.uint32)
+    if g.ndim != 2 or g.shape[1] != 3 or g.dtype.kind not in "iu" or g.min() < 0 or g.max() > 0xFFFFFFFF:
+        raise ValueError("prefix groups are (first row, rows, prefix pages)")
+    return np.ascontiguousarray(g, dtype=np.uint32)
+
+
 class TpBatchRunner:
     """One-GPU runner behind the reference's batch-runner boundary."""
 
@@ -233,15 +243,23 @@ class TpBatchRunner:
     def row_capacity(self) -> int:
         return int(self._lib.fh_row_capacity(self._ctx))
 
-    def execute_batch(self, batch: PreparedBatch, output_rows: Sequence[int]) -> BatchOutput:
+    def execute_batch(self, batch: PreparedBatch, output_rows: Sequence[int], prefix_groups=()) -> BatchOutput:
+        """One step. prefix_groups: [(first row, rows, prefix pages)] of a decode
+        batch whose rows share prefixes (PagePool.prefix_groups), whose pages
+        the attention then reads once a group (fh_execute_batch_shared)."""
         if batch.limits != self.limits:
             raise FerricError(2, "foreign, stale, or invalid prepared GPU batch")
         rows, keep = _rows_to_c(batch.rows)
         outs = np.ascontiguousarray(np.asarray(output_rows, dtype=np.uint32))
         choices = np.zeros(max(len(outs), 1), dtype=np.uint32)
-        st = self._lib.fh_execute_batch(self._ctx, batch.id, rows, len(batch.rows),
-                                        outs.ctypes.data_as(ctypes.POINTER(ctypes.c_uint32)), len(outs),
-                                        choices.ctypes.data_as(ctypes.POINTER(ctypes.c_uint32)))
+        outs_p = outs.ctypes.data_as(ctypes.POINTER(ctypes.c_uint32))
+        choices_p = choices.ctypes.data_as(ctypes.POINTER(ctypes.c_uint32))
+        if len(prefix_groups):
+            groups = _groups_to_c(prefix_groups)
+            st = self._lib.fh_execute_batch_shared(self._ctx, batch.id, rows, len(batch.rows), groups.ctypes.data,
+                                                   len(groups), outs_p, len(outs), choices_p)
+        else:
+            st = self._lib.fh_execute_batch(self._ctx, batch.id, rows, len(batch.rows), outs_p, len(outs), choices_p)
         del keep
         check(st, self._ctx)
         # Decode batches produce logits for every row, prefill chunks for the output rows only.
@@ -252,8 +270,9 @@ class TpBatchRunner:
     def output_head_rows(self, physical: int, published: int) -> int:
         return physical
 
-    def expected_dispatch_counts_for_selection(self, batch: PreparedBatch, output_rows: Sequence[int]) -> list:
-        """The dispatch_counts() increment execute_batch(batch, output_rows) will
+    def expected_dispatch_counts_for_selection(self, batch: PreparedBatch, output_rows: Sequence[int],
+                                               prefix_groups=()) -> list:
+        """The dispatch_counts() increment execute_batch with these arguments will
         make (one entry: one context stands in for every rank), evaluated by
         the library without launching (fh_expected_dispatch_count). Raises the
         execute_batch error for a batch it would reject."""
@@ -262,9 +281,10 @@ class TpBatchRunner:
         rows, keep = _rows_to_c(batch.rows)
         outs = np.ascontiguousarray(np.asarray(output_rows, dtype=np.uint32))
         count = ctypes.c_uint64()
-        st = self._lib.fh_expected_dispatch_count(self._ctx, batch.id, rows, len(batch.rows),
-                                                  outs.ctypes.data_as(ctypes.POINTER(ctypes.c_uint32)), len(outs),
-                                                  ctypes.byref(count))
+        groups = _groups_to_c(prefix_groups)
+        st = self._lib.fh_expected_dispatch_count_shared(self._ctx, batch.id, rows, len(batch.rows), groups.ctypes.data,
+                                                         len(groups), outs.ctypes.data_as(ctypes.POINTER(ctypes.c_uint32)),
+                                                         len(outs), ctypes.byref(count))
         del keep
         check(st, self._ctx)
         return [int(count.value)]

@@ -175,6 +175,27 @@ fh_status fh_kv_copy_pages(fh_ctx* ctx, const fh_kv_move* moves, uint32_t count)
 fh_status fh_execute_batch(fh_ctx* ctx, uint64_t batch_id, const fh_row* rows, uint32_t nrows,
                            const uint32_t* output_rows, uint32_t nout, uint32_t* choices_out);
 
+/* Rows [first_row, first_row + rows) of a batch whose page tables agree in their first
+ * prefix_pages entries: continuations of one prompt (forks), or rows of one sequence. */
+typedef struct fh_prefix_group {
+  uint32_t first_row;
+  uint32_t rows;
+  uint32_t prefix_pages;
+} fh_prefix_group;
+
+/* fh_execute_batch for a decode batch (nrows <= row_capacity) whose rows share prefixes
+ * (continuations of one prompt): the attention reads the pages of a group's prefix once for
+ * its rows (fh_op_prefix_attention) instead of once a row; the logits differ from
+ * fh_execute_batch's by the order of sums only. groups: as fh_op_prefix_attention, each with
+ * prefix_pages >= 1 whole pages that every row of it lists at the start of its list and
+ * writes behind; else FH_ERR_INVALID_ARGUMENT, and nothing has run. ngroups 0:
+ * fh_execute_batch itself. A second step with the same rows and groups is captured into a
+ * graph, later ones replay it. The scratch is the context's and grows on demand
+ * (FH_ERR_OUT_OF_MEMORY, nothing has run). No counterpart in the reference. */
+fh_status fh_execute_batch_shared(fh_ctx* ctx, uint64_t batch_id, const fh_row* rows, uint32_t nrows,
+                                  const fh_prefix_group* groups, uint32_t ngroups, const uint32_t* output_rows,
+                                  uint32_t nout, uint32_t* choices_out);
+
 /* Parity readbacks of the last batch: FP32 logits [nrows][vocabulary] (prefill: the
  * output rows, in output order); the residual stream after layer `layer`
  * [nrows][hidden] for every token row of the batch (needs capture_hidden, which
@@ -197,6 +218,10 @@ uint64_t fh_dispatch_count(const fh_ctx* ctx);
  * whose result the caller compares with the dispatch_counts() increment (tp_batch_runtime.rs:432-446). */
 fh_status fh_expected_dispatch_count(fh_ctx* ctx, uint64_t batch_id, const fh_row* rows, uint32_t nrows,
                                      const uint32_t* output_rows, uint32_t nout, uint64_t* count);
+/* The same for fh_execute_batch_shared (9 launches per layer for more than one row). */
+fh_status fh_expected_dispatch_count_shared(fh_ctx* ctx, uint64_t batch_id, const fh_row* rows, uint32_t nrows,
+                                            const fh_prefix_group* groups, uint32_t ngroups,
+                                            const uint32_t* output_rows, uint32_t nout, uint64_t* count);
 /* Device milliseconds of the last fh_execute_batch, from HIP events on the context stream. */
 float fh_last_step_ms(const fh_ctx* ctx);
 /* Per-kernel-class device time of the last batch when profiling is on (parity/bench aid).
@@ -204,7 +229,8 @@ float fh_last_step_ms(const fh_ctx* ctx);
 fh_status fh_set_profiling(fh_ctx* ctx, uint32_t enabled);
 fh_status fh_kernel_class_ms(const fh_ctx* ctx, uint32_t kernel_class, float* ms, uint32_t* launches);
 /* Measurement aid with no counterpart in the reference: re-launches the last decode
- * batch's attention partition kernel for the last layer (same inputs, so it rewrites the
+ * batch's attention partition kernel (or, for rows that shared prefixes, that attention's two
+ * launches) for the last layer (same inputs, so it rewrites the
  * same outputs) reps times back to back on the context stream between two events and
  * writes the mean launch duration in ms (1 <= reps <= 1000). FH_ERR_STATE if the last
  * batch was not a decode batch. */
@@ -412,14 +438,6 @@ fh_status fh_op_paged_attention_noalloc(const uint16_t* q, const uint16_t* k_cac
                                         uint32_t out_tiled, uint32_t rows, uint32_t query_heads, uint32_t kv_heads,
                                         uint32_t stride, uint32_t physical_pages, uint32_t context_tokens,
                                         uint32_t* error_word, void* stream);
-
-/* Rows [first_row, first_row + rows) of a batch whose page tables agree in their first
- * prefix_pages entries: continuations of one prompt (forks), or rows of one sequence. */
-typedef struct fh_prefix_group {
-  uint32_t first_row;
-  uint32_t rows;
-  uint32_t prefix_pages;
-} fh_prefix_group;
 
 /* K4 for such batches: fh_op_paged_attention's result, with each group's prefix (16 x
  * prefix_pages tokens) read once for all of its rows instead of once per row, and each row's
