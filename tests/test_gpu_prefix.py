@@ -164,6 +164,71 @@ def test_several_rows_of_a_sequence(per, own):
     holds(b, bits)
 
 
+@pytest.mark.parametrize("heads", [(32, 8), (16, 8), (8, 8), (64, 8), (4, 4)])
+@pytest.mark.parametrize("per,own", [(3, 3), (4, 18), (5, 600), (9, 33), (17, 1500), (17, 17)])
+def test_runs_of_rows_of_one_sequence(per, own, heads):
+    """Runs that end inside and at the rows taken together, that cross pages, and whose keys are cut into parts."""
+    b = Batch(per + own, [([own, own + 15], 3), ([own + 2], 0), ([per], 1)], *heads, per=per).device()
+    bits, err = b.run()
+    assert err == 0
+    holds(b, bits)
+
+
+def test_consecutive_positions_of_different_sequences():
+    b = Batch(30, [([40, 41, 42, 43, 44], 2), ([16, 17, 18], 0), ([1, 2, 3, 4], 1), ([0, 1, 2], 3)], 32, 8)
+    # Row 2's list like row 1's from its third own page on, and row 4's like row 3's but for the prefix's successor.
+    b.table[2, 4:] = b.table[1, 4:]
+    swap = [p for p in range(b.pages) if p not in b.table][0]
+    b.k[swap], b.v[swap] = b.k[int(b.table[3, 2])] * 2, b.v[int(b.table[3, 2])] + 1
+    b.table[4] = b.table[3]
+    b.table[4, 2] = swap
+    for r in (1, 3):  # the slots of the later rows' last positions
+        page = int(b.table[r, 4])
+        b.k[page, 8:13] = b.k[page, :5]
+        b.v[page, 8:13] = b.v[page, :5]
+    bits, err = b.device().run()
+    assert err == 0
+    holds(b, bits)
+
+
+@pytest.mark.parametrize("heads", [(32, 8), (8, 8)])
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("bad", [NAN, float("inf")])
+def test_a_later_rows_nonfinite_slot_does_not_reach_the_earlier_rows(bad, which, heads):
+    b = Batch(31, [([37], 2)], *heads, per=6)  # positions 63..68
+    page = int(b.table[0, 66 // 16])
+    (b.k if which == "k" else b.v)[page, 66 % 16, :, 11] = bad
+    bits, err = b.device().run()
+    assert err == NONFINITE
+    holds(b, bits, [0, 1, 2])
+    got = values(bits, b)
+    # An infinite key against a negative query component has the score -inf, the weight 0 and a finite row.
+    hit = b.q[3:, :, 11] > 0 if which == "k" and bad == float("inf") else torch.ones(3, heads[0], dtype=torch.bool)
+    assert not torch.isfinite(got[3:, :, 11])[hit].any()
+
+
+def test_a_later_row_whose_own_key_scores_minus_infinity_is_reported():
+    b = Batch(33, [([37], 2)], 8, 8, per=6)
+    b.q[3:, :, 11] = -1
+    b.k[int(b.table[0, 66 // 16]), 66 % 16, :, 11] = float("inf")
+    bits, err = b.device().run()
+    assert err == NONFINITE
+    holds(b, bits, [0, 1, 2])
+
+
+def test_a_run_with_a_position_or_page_out_of_range_in_its_midst():
+    b = Batch(32, [([50], 2)], 32, 8, per=8).device()
+    b.d["pos"][3] = b.context
+    bits, err = b.run()
+    assert err == POSITION
+    holds(b, bits, [0, 1, 2, 4, 5, 6, 7])
+    b = Batch(32, [([50], 2)], 32, 8, per=8)  # lengths 75..82: the last two rows begin page 5
+    b.table[7, 5] = b.pages
+    bits, err = b.device().run()
+    assert err == PAGE
+    holds(b, bits, range(7))
+
+
 def test_sixty_four_groups_of_one_row_and_empty_ones():
     b = Batch(1, [([1 + i % 40], 1 + i % 3) for i in range(64)], 16, 8).device()
     bits, err = b.run()
