@@ -732,12 +732,13 @@ struct PrefixPlan {
 PrefixPlan prefix_plan(const fh_prefix_group* groups, uint32_t ngroups, uint32_t rows, uint32_t qh, uint32_t kvh) {
   PrefixPlan p{};
   const uint32_t g = qh / kvh;
-  uint32_t most = 0;
+  uint32_t most = 0, longest = 0;
   for (uint32_t i = 0; i < ngroups; ++i) {
     if (groups[i].prefix_pages == 0) continue;
     Group& to = p.gs.g[p.gs.count++];
     to = Group{groups[i].first_row, groups[i].rows, groups[i].prefix_pages * 16, 0};
     if (to.rows > most) most = to.rows;
+    if (to.prefix_tokens > longest) longest = to.prefix_tokens;
   }
   const uint64_t vectors = (uint64_t)most * g;
   if (most == 0) most = 1;
@@ -756,6 +757,7 @@ PrefixPlan prefix_plan(const fh_prefix_group* groups, uint32_t ngroups, uint32_t
   p.gs.block_rows = (p.form == 1 ? 128 : p.form == 2 ? 64 : kVectors) / g;
   p.gs.stream = most <= p.gs.block_rows && tokens_of(most) * 512 >= kStreamBytes;
   uint64_t chunk = (tokens_of(p.gs.block_rows) / kChunkWgs + 63) / 64 * 64;
+  if (chunk > longest) chunk = (longest + 63) / 64 * 64;  // (many rows and heads: tokens_of may pass 2^40)
   if (chunk < kMinChunk) chunk = kMinChunk;
   p.gs.chunk = (uint32_t)chunk;
   for (uint32_t i = 0; i < p.gs.count; ++i) {

@@ -28,14 +28,17 @@ inline bool aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<u
 
 // Head counts of the attention kernels and sizes whose products fit the launch.
 inline bool prefix_shape_ok(uint32_t rows, uint32_t qh, uint32_t kvh, uint32_t context) {
-  if (rows == 0 || rows > 65535u || kvh == 0 || kvh > 4096u || qh % kvh != 0 || context == 0 || context > 1u << 24)
+  // (A launch holds 2^32 threads: 512 a row and KV head.)
+  if (rows == 0 || rows > 65535u || kvh == 0 || kvh > 4096u || (uint64_t)rows * kvh > 1u << 22 || qh % kvh != 0 || context == 0 || context > 1u << 24)
     return false;
   const uint32_t g = qh / kvh;
   return g == 1 || g == 2 || g == 4 || g == 8;
 }
 
+// (A launch holds 2^32 threads: one for eight weights of the quantizer.)
+inline bool w4_size_ok(uint32_t n, uint32_t k) { return (uint64_t)n * k < 1ull << 35; }
 inline bool w4_shape_ok(uint32_t n, uint32_t k, uint32_t group) {
-  return n != 0 && k != 0 && n % 16 == 0 && k % 128 == 0 && k <= 1u << 24 && (group == 32 || group == 64 || group == 128);
+  return n != 0 && k != 0 && n % 16 == 0 && k % 128 == 0 && k <= 1u << 24 && w4_size_ok(n, k) && (group == 32 || group == 64 || group == 128);
 }
 
 #define from_hip(expr) (static_cast<void>(hipGetLastError()), status_of(expr))
@@ -177,7 +180,7 @@ fh_status fh_op_gemm_w4(const uint16_t* x_tiled, const uint32_t* w_tiled, const 
 
 fh_status fh_op_quantize_w4(const uint16_t* src, uint8_t* packed, uint16_t* scales, uint32_t n, uint32_t k,
                             uint32_t group, uint32_t* error_word, void* stream) {
-  if (!src || !packed || !scales || n == 0 || !w4_shape_ok(16, k, group) || (uint64_t)n * k > 1ull << 40 ||
+  if (!src || !packed || !scales || n == 0 || !w4_shape_ok(16, k, group) || !w4_size_ok(n, k) ||
       !aligned(src, 16) || !aligned(packed, 4))
     return FH_ERR_INVALID_ARGUMENT;
   return from_hip(fh::launch_quantize_w4(src, packed, scales, n, k, group, error_word, as_stream(stream)));
@@ -187,7 +190,7 @@ fh_status fh_op_tile_weight_w4(const uint8_t* packed, const uint16_t* scales, co
                                uint32_t* w_tiled, uint16_t* scales_tiled, uint8_t* zeros_tiled, uint32_t n, uint32_t k,
                                uint32_t group, uint32_t part, void* stream) {
   if (!packed || !scales || !w_tiled || !scales_tiled || (zeros && !zeros_tiled) || !w4_shape_ok(n, k, group) ||
-      (uint64_t)n * k > 1ull << 40 || part > 2 || !aligned(packed, 4) || !aligned(w_tiled, 16))
+      part > 2 || !aligned(packed, 4) || !aligned(w_tiled, 16))
     return FH_ERR_INVALID_ARGUMENT;
   return from_hip(fh::launch_tile_weight_w4(packed, scales, zeros, w_tiled, scales_tiled, zeros_tiled, n, k, group,
                                             part ? 2 : 1, part == 2 ? 1 : 0, as_stream(stream)));

@@ -298,10 +298,11 @@ fh_status fh_op_gemm(const uint16_t* x_tiled, const uint16_t* w_tiled, uint32_t 
 /* K1 projections with 4-bit weights and group scales, for decode batches (1 <= m <= 32):
  * out = epilogue(x[m][k] . W[n][k]^T), W[n][k] = scale[n][k / group] * (q[n][k] - zero[n][k / group]),
  * q in 0..15, zero 8 where zeros_tiled is NULL; FP32 accumulation on MFMA (the quantized
- * weights enter it exactly). n % 16 == 0 (32 for FH_EPI_SWIGLU), k % 128 == 0, k <= 2^24, group
- * 32, 64 or 128. Epilogues, x_tiled, splits (<= k / 128 and 65535), residual, out, ldo and error_word as
- * fh_op_gemm; only the first m rows of out are written. Operands in the order
- * fh_op_tile_weight_w4 writes, w_tiled and x_tiled 16-byte, scales_tiled 8-byte and
+ * weights enter it exactly, as 16 + q: a row whose activations' absolute values add up to more
+ * than 2^122 in a group, or that holds an infinity, may give NaN). n % 16 == 0 (32 for
+ * FH_EPI_SWIGLU), k % 128 == 0, k <= 2^24, n * k < 2^35, group 32, 64 or 128. Epilogues,
+ * x_tiled, splits (<= k / 128 and 65535), residual, out, ldo and error_word as fh_op_gemm; only
+ * the first m rows of out are written. Operands in the order fh_op_tile_weight_w4 writes, w_tiled and x_tiled 16-byte, scales_tiled 8-byte and
  * zeros_tiled 4-byte aligned. No counterpart in the reference, whose projections read bf16
  * weights (gemm.rs:161/:605). */
 fh_status fh_op_gemm_w4(const uint16_t* x_tiled, const uint32_t* w_tiled, const uint16_t* scales_tiled,
@@ -313,7 +314,7 @@ uint32_t fh_gemm_w4_default_splits(uint32_t n, uint32_t k);
 /* Rounds a row-major bf16 weight [n][k] to 4 bits per group (symmetric: no zero points):
  * scale = bf16(max |w| / 7), q = 8 + clamp(rne(w / scale), -8, 7), 8 where the scale is 0.
  * packed: [n][k / 2] bytes, even columns in the low half; scales: [n][k / group] bf16. k and
- * group as fh_op_gemm_w4, n * k <= 2^40; src 16-byte, packed 4-byte aligned. error_word (may be
+ * group as fh_op_gemm_w4, n * k < 2^35; src 16-byte, packed 4-byte aligned. error_word (may be
  * NULL) receives the nonfinite bit where the weight holds a nonfinite value. */
 fh_status fh_op_quantize_w4(const uint16_t* src, uint8_t* packed, uint16_t* scales, uint32_t n, uint32_t k,
                             uint32_t group, uint32_t* error_word, void* stream);
@@ -443,8 +444,8 @@ fh_status fh_op_paged_attention_noalloc(const uint16_t* q, const uint16_t* k_cac
  * prefix_pages tokens) read once for all of its rows instead of once per row, and each row's
  * other keys once for the row. groups is host memory, read before the call returns (a
  * captured graph keeps them): 0..64 groups, ascending and disjoint; rows in no group share
- * nothing. Up to 65535 rows and 2^24 context tokens; several rows may belong to one sequence. Every row of a group has
- * position >= 16 x prefix_pages - 1 (its prefix is all visible; ERR_POSITION in error_word
+ * nothing. Up to 65535 rows (2^22 with their KV heads) and 2^24 context tokens; several rows may
+ * belong to one sequence. Every row of a group has position >= 16 x prefix_pages - 1 (its prefix is all visible; ERR_POSITION in error_word
  * and no output for the row otherwise), and its table's first prefix_pages entries are those
  * of the group's first row (the page bit of error_word otherwise). q, out, out_tiled, tables
  * and errors as fh_op_paged_attention; q and the caches 16-byte, out 8-byte aligned. scratch:

@@ -57,6 +57,13 @@ def test_scratch_is_asked_for_and_checked():
     n = LIB.fh_prefix_attention_scratch_bytes(g.ctypes.data, 1, 4, 32, 8, 128)
     assert n > 0 and call(g, nbytes=n - 1) == 1
     assert LIB.fh_prefix_attention_scratch_bytes(None, 0, 4, 32, 8, 128) > 0
-    for rows, qh, kvh, context in [(0, 32, 8, 128), (4, 31, 8, 128), (4, 32, 0, 128), (4, 32, 8, 0)]:
+    for rows, qh, kvh, context in [(0, 32, 8, 128), (65535, 65, 65, 128), (65536, 8, 8, 128), (4, 31, 8, 128), (4, 32, 0, 128), (4, 32, 8, 0)]:
         assert LIB.fh_prefix_attention_scratch_bytes(None, 0, rows, qh, kvh, context) == 0
     assert ctypes.sizeof(_lib.PrefixGroup) == 12
+
+
+@pytest.mark.parametrize("rows,qh,kvh", [(65535, 128, 16), (65535, 512, 64), (1024, 32768, 4096), (1, 4096, 4096)])
+def test_scratch_of_the_largest_batches(rows, qh, kvh):
+    g = groups_of((0, rows, 1 << 20))
+    n = LIB.fh_prefix_attention_scratch_bytes(g.ctypes.data, 1, rows, qh, kvh, 1 << 24)
+    assert n >= rows * qh * 132 * 4  # a record a query head at least

@@ -15,7 +15,7 @@ def gemm(x=P, w=P, s=P, z=None, m=1, n=32, k=256, group=64, epi=0, splits=1, res
     return LIB.fh_op_gemm_w4(x, w, s, z, m, n, k, group, epi, splits, residual, out, ldo, None, None)
 
 
-@pytest.mark.parametrize("bad", [dict(x=None), dict(w=None), dict(s=None), dict(out=None), dict(m=0), dict(m=33), dict(k=(1 << 24) + 128), dict(n=0),
+@pytest.mark.parametrize("bad", [dict(x=None), dict(w=None), dict(s=None), dict(out=None), dict(m=0), dict(m=33), dict(k=(1 << 24) + 128), dict(n=2**31, k=128, ldo=2**31), dict(n=0),
                                  dict(n=24), dict(k=0), dict(k=192), dict(group=16), dict(group=256), dict(group=0),
                                  dict(epi=5), dict(splits=0), dict(splits=2), dict(epi=4, splits=3), dict(epi=1), dict(ldo=31),
                                  dict(epi=2, n=16), dict(x=P + 8), dict(w=P + 8), dict(s=P + 4), dict(z=P + 2),
@@ -25,7 +25,7 @@ def test_gemm_refusals(bad):
 
 
 @pytest.mark.parametrize("bad", [dict(n=0), dict(k=64), dict(k=0), dict(group=48), dict(src=None), dict(packed=None),
-                                 dict(scales=None), dict(src=P + 2), dict(packed=P + 1), dict(n=2**31, k=1024)])
+                                 dict(scales=None), dict(src=P + 2), dict(packed=P + 1), dict(n=2**28, k=128)])
 def test_quantize_refusals(bad):
     a = dict(src=P, packed=P, scales=P, n=16, k=128, group=32) | bad
     assert LIB.fh_op_quantize_w4(a["src"], a["packed"], a["scales"], a["n"], a["k"], a["group"], None, None) == 1
@@ -33,7 +33,7 @@ def test_quantize_refusals(bad):
 
 @pytest.mark.parametrize("bad", [dict(n=8), dict(k=64), dict(group=96), dict(packed=None), dict(scales=None), dict(w=None),
                                  dict(st=None), dict(z=P, zt=None), dict(part=3), dict(packed=P + 2), dict(w=P + 8),
-                                 dict(n=2**31, k=1024)])
+                                 dict(n=2**28, k=128)])
 def test_tile_refusals(bad):
     a = dict(packed=P, scales=P, z=None, w=P, st=P, zt=None, n=16, k=128, group=32, part=0) | bad
     assert LIB.fh_op_tile_weight_w4(a["packed"], a["scales"], a["z"], a["w"], a["st"], a["zt"], a["n"], a["k"], a["group"],
