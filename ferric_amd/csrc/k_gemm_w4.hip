@@ -28,10 +28,10 @@
 //
 // What bounds it: the weights' bytes from HBM in 7 rows through 151936 x 4096 (60
 // us, 325 MB at 5.4 TB/s, the rate of a large copy); a launch's start and end beside them
-// in one row through 24576 x 4096 (12.3 us, 52 MB; 9.6 at that rate). From about 16
+// in one row through 24576 x 4096 (11.9 us, 52 MB; 9.6 at that rate). From about 16
 // rows on, and with few weight rows a workgroup, the activations, which every workgroup
 // reads whole from the L2: 32 rows through 4096 x 12288 take 786 KB into each CU
-// beside 115 KB of weights, 16.2 us, and 10.8 with those loads left out.
+// beside 115 KB of weights, 15.2 us, and 12.2 with one in six of those loads made.
 #include "common.hpp"
 #include "kernels.hpp"
 
@@ -42,13 +42,13 @@ namespace {
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 
 // Waves of a workgroup, which divide its k: 4 where there are kMany workgroups (one row through 24576 x 4096
-// in 768 of them: 12.2 us, 13.1 with 16 waves, 14.7 with 8), else 16 (4 rows through 4096 x 4096 in 256: 4.7 us,
+// in 768 of them: 11.9 us, 13.1 with 16 waves, 14.7 with 8), else 16 (4 rows through 4096 x 4096 in 256: 4.7 us,
 // 5.7 with 8, 8.6 with 4; 1024 x 2048 in 64: 2.9, 3.0, 3.6).
 constexpr uint32_t kMany = 512;
 constexpr int kWavesFew = 16, kWavesMany = 4;
 // Weight tiles of a workgroup, which share its activations: 4 where enough workgroups are left (7 rows through
-// 151936 x 4096 60 us, 67 with 2; 32 rows through 24576 x 4096 17.8, 18.8). One row asks for more of them: through
-// 24576 x 4096 12.9, with 2 tiles 12.2.
+// 151936 x 4096 60 us, 67 with 2; 32 rows through 24576 x 4096 17.5, 18.8). One row asks for more of them: through
+// 24576 x 4096 12.9, with 2 tiles 11.9.
 constexpr uint32_t kQuadFrom = 1024, kQuadFromWide = 256, kPairFrom = 256;
 
 __device__ __forceinline__ bf16x8 unpack_w4(uint32_t w, uint32_t mask, uint32_t base) {
@@ -63,13 +63,18 @@ __device__ __forceinline__ bf16x8 unpack_w4(uint32_t w, uint32_t mask, uint32_t 
 // through LDS. GB: 32-column k-blocks per group. MT: 16-row activation tiles.
 // A wave has one block in flight and leaves the rest to the other waves of its SIMD, up to 8:
 // with two or three in flight, which take the registers of as many waves, nothing was
-// faster (32 rows through 24576 x 4096: 20.3 us with two, 17.8 with one).
+// faster (32 rows through 24576 x 4096: 20.3 us with two, 17.5 with one). But where few
+// workgroups take more than 16 rows, each wave's turns are few and long, and the weights of
+// kAhead blocks are requested before the activations of the first (32 rows through 4096 x
+// 12288: 15.2 us, 16.4 without; through 4096 x 4096 6.5, 7.0; one row through 4096 x
+// 12288 8.1 without, 8.5 with it).
 template <int NT, int MT, int GB, bool ZP, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, WAVES == 4 && (NT == 4 || MT == 2) ? 3 : 4) void gemm_w4_kernel(
     const uint16_t* __restrict__ xt, const uint32_t* __restrict__ w, const uint16_t* __restrict__ scales,
     const uint8_t* __restrict__ zeros, uint32_t m, uint32_t kb_count, uint32_t kb_split, uint32_t epi,
     const uint16_t* residual, void* out, uint32_t ldo, uint32_t* err) {
   constexpr int GP = 4 / GB;  // groups per 128 columns
+  constexpr int kAhead = WAVES == kWavesFew && MT == 2 ? (NT == 1 ? 3 : 2) : 1;
   __shared__ float red[WAVES][NT * MT * 256];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t tile0 = blockIdx.x * NT, split = blockIdx.y;
@@ -77,8 +82,8 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 && (NT == 4 || MT == 2) ? 3 
   const uint32_t kb_lo = s_lo + (s_n * wave) / WAVES, kb_hi = s_lo + (s_n * (wave + 1)) / WAVES;
   const uint32_t r16 = lane & 15, g16 = lane >> 4;
 
-  struct Block {
-    u32x4 w[NT], x[4][MT];
+  struct Weights {  // of 128 columns
+    u32x4 w[NT];
     uint32_t s[NT];           // scale of row lane % 16, group lane / 16 % GP
     uint32_t z[ZP ? NT : 1];  // its zero point
   };
@@ -94,13 +99,15 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 && (NT == 4 || MT == 2) ? 3 
   uint32_t xoff[MT];
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) xoff[mt] = mt * 1024 + (min(16 * mt + r16, m - 1) & 15u) * 16 + g16 * 256;
-  auto load = [&](Block& b, uint32_t kb) {
+  auto load_x = [&](u32x4 (&x)[4][MT], uint32_t kb) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
-        b.x[j][mt] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                                                    xr, xoff[mt] + (j & 1) * 2048, kb * 8192 + (j >> 1) * 4096, 0));
+        x[j][mt] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                 xr, xoff[mt] + (j & 1) * 2048, kb * 8192 + (j >> 1) * 4096, 0));
+  };
+  auto load_w = [&](Weights& b, uint32_t kb) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       b.w[nt] = __builtin_bit_cast(
@@ -124,7 +131,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 && (NT == 4 || MT == 2) ? 3 
   // bf16 -16 (with zero points) or -24.
   constexpr uint32_t kOff = ZP ? 0xc180c180u : 0xc1c0c1c0u;
   const bf16x8 offset = __builtin_bit_cast(bf16x8, u32x4{kOff, kOff, kOff, kOff});
-  auto compute = [&](const Block& b) {
+  auto compute = [&](const Weights& b, const u32x4 (&x)[4][MT]) {
     // Scale (low half) and zero point of a group in all lanes of its row: the lanes' words, their 16-lane groups
     // exchanged.
     uint32_t sz[NT][GP];
@@ -156,7 +163,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 && (NT == 4 || MT == 2) ? 3 
         sx[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < GB; ++i)
-          sx[mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b.x[p * GB + i][mt]), offset,
+          sx[mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x[p * GB + i][mt]), offset,
                                                            sx[mt], 0, 0, 0);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) part[nt][mt] = sx[mt];
@@ -169,7 +176,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 && (NT == 4 || MT == 2) ? 3 
           const bf16x8 q = unpack_w4(b.w[nt][j], mask, base);
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt)
-            part[nt][mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b.x[j][mt]), q,
+            part[nt][mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x[j][mt]), q,
                                                                   part[nt][mt], 0, 0, 0);
         }
       }
@@ -189,11 +196,19 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 && (NT == 4 || MT == 2) ? 3 
       }
     }
   };
-  for (uint32_t kb = kb_lo; kb < kb_hi; ++kb) {
-    Block b;
-    load(b, kb);
-    __builtin_amdgcn_sched_barrier(0);  // all of the block's loads are on their way before the first wait
-    compute(b);
+  for (uint32_t kb = kb_lo; kb < kb_hi; kb += kAhead) {
+    Weights b[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (i == 0 || kb + i < kb_hi) load_w(b[i], kb + i);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (i != 0 && kb + i >= kb_hi) break;
+      u32x4 x[4][MT];
+      load_x(x, kb + i);
+      __builtin_amdgcn_sched_barrier(0);  // all loads are on their way before the first wait
+      compute(b[i], x);
+    }
   }
 
 #pragma unroll
