@@ -38,8 +38,9 @@
 // the next fetch. Narrow (own keys, and prefix chunks of up to 16 vectors): the waves
 // take 32 keys each, K straight into the A operand's registers (a token's 64-byte
 // pieces), V through 8 KiB of LDS of the wave's own; their states meet in LDS at the
-// end. All forms keep to 128 registers a thread and 67.6 KB of LDS, so that two
-// workgroups share a CU and one computes while the other waits.
+// end. All forms keep to 128 registers a thread and 67.6 KB of LDS (own keys in
+// workgroups of 4 waves to half of it), so that two workgroups (four) share a CU and
+// one computes while the other waits.
 //
 // What bounds it (kernel times, 32 rows, 8 KV heads of 4 query heads): behind 8192
 // shared tokens the first launch takes 15 us (33.6 MB of keys and values, which the
@@ -65,7 +66,6 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 constexpr int kWaves = 8;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kKeys = 64;             // keys per tile of the wide form
-constexpr int kStep = 32 * kWaves;    // keys of the narrow form's waves at once
 constexpr size_t kTileBytes = 16 * 2 * kKeys * 16;  // K or V, double-buffered
 // Least tokens of a prefix chunk (256 instead: 4 rows behind 1488 tokens 1.1 us slower).
 constexpr uint32_t kMinChunk = 128;
@@ -76,11 +76,16 @@ constexpr uint32_t kChunkWgs = 256;
 // behind 32000 tokens, 131 MB: 61.7 us cached, 53.2 streamed; smaller ones, which the
 // 256 MB cache still holds from the step before, are 3 to 10 % slower streamed).
 constexpr uint64_t kStreamBytes = 96ull << 20;
-// Least own keys of a part where a row has several. A step of kStep keys takes about 3.5 us and the
+// Least own keys of a part where a row has several. A step of 256 keys takes about 3.5 us and the
 // meeting of the parts about 3: with few (row, KV head) pairs 256 (2 rows of 2000 own keys:
 // 18.9 us, with 512 21.0, with 1024 29.4), with many, where parts only take turns, 512
 // (29 rows of up to 900: 25.8 us with 256, 24.5 with 512).
 constexpr uint32_t kPartKeysFew = 256, kPartKeysMany = 512, kManyPairs = 128;
+// Own keys in workgroups of 4 waves, four on a CU, where there are this many (row, KV head) pairs and none can have
+// more than kShortOwn own keys (160 rows of 8 KV heads with up to 300: 42.6 us, with 8 waves 47.6; 64 rows
+// with up to 60: 14.2, 15.3); a longest row sets the time else, and 8 waves are through with it
+// sooner (80 rows with up to 1500: 39.6 us, with 4 waves 44.5; 128 with 500 to 2000: 97.4, 102.6).
+constexpr uint32_t kManyOwn = 512, kShortOwn = 512;
 constexpr uint32_t kMaxParts = 32;
 constexpr uint32_t kSlots = 512;      // workgroups that run at once: two on each CU
 constexpr uint32_t kVectors = 16;     // of a wave
@@ -445,19 +450,24 @@ __device__ __forceinline__ Part join_all(const Part& t, const Part (&x)[N]) {
 
 // LDS of the narrow form: V of each wave's 32 keys, then the waves' states.
 // (Rows of 528 bytes keep the accumulators' stores off each other's banks.)
+template <int NW>
 struct NarrowState {
-  float acc[kWaves][kVectors][132];
+  float acc[NW][kVectors][132];
 };
-static_assert(sizeof(NarrowState) >= 2 * kTileBytes, "and the wide form's tiles fit too");
+static_assert(sizeof(NarrowState<kWaves>) >= 2 * kTileBytes, "and the wide form's tiles fit too");
+static_assert(sizeof(NarrowState<1>) >= 32 * 256, "and a wave's V");
+template <int NW>
 struct NarrowSums {
-  float m[kWaves][kVectors], l[kWaves][kVectors];  // m in the exponent of 2
+  float m[NW][kVectors], l[NW][kVectors];  // m in the exponent of 2
 };
 
-// The narrow form: as above for nrows * G <= 16 vectors; the waves' states are left in LDS, behind a barrier.
-template <int G>
-__device__ __forceinline__ void attend_narrow(unsigned char* lds_raw, NarrowSums& sums, const Args& a,
+// The narrow form: as above for nrows * G <= 16 vectors and NW waves; their states are left in LDS, behind a
+// barrier.
+template <int G, int NW>
+__device__ __forceinline__ void attend_narrow(unsigned char* lds_raw, NarrowSums<NW>& sums, const Args& a,
                                               const uint32_t* __restrict__ trow, uint32_t row0, uint32_t nrows,
                                               uint32_t key0, uint32_t key1, uint32_t h) {
+  constexpr uint32_t kStep = 32 * NW;  // keys of the waves at once
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   u32x4(*vlds)[16] = reinterpret_cast<u32x4(*)[16]>(lds_raw) + 32 * wave;
   const uint32_t page0 = key0 / 16, npages = (key1 - key0 + 15) / 16, steps = (key1 - key0 + kStep - 1) / kStep;
@@ -524,7 +534,7 @@ __device__ __forceinline__ void attend_narrow(unsigned char* lds_raw, NarrowSums
   }
   st.finish();
   __syncthreads();  // every wave is done with its V
-  auto& all = *reinterpret_cast<NarrowState*>(lds_raw);
+  auto& all = *reinterpret_cast<NarrowState<NW>*>(lds_raw);
   const uint32_t vec = lane & 15;
   if (vec < nrows * G) {
 #pragma unroll
@@ -540,13 +550,14 @@ __device__ __forceinline__ void attend_narrow(unsigned char* lds_raw, NarrowSums
 }
 
 // The waves' states of vector v, dims 4 c .. 4 c + 3, joined in wave order (the maximum first, then one sum).
-__device__ __forceinline__ Part narrow_part(unsigned char* lds_raw, const NarrowSums& sums, uint32_t v, uint32_t c) {
-  auto& all = *reinterpret_cast<NarrowState*>(lds_raw);
+template <int NW>
+__device__ __forceinline__ Part narrow_part(unsigned char* lds_raw, const NarrowSums<NW>& sums, uint32_t v, uint32_t c) {
+  auto& all = *reinterpret_cast<NarrowState<NW>*>(lds_raw);
   Part o = no_part();
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) o.m = fmaxf(o.m, sums.m[w][v]);
+  for (int w = 0; w < NW; ++w) o.m = fmaxf(o.m, sums.m[w][v]);
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
+  for (int w = 0; w < NW; ++w) {
     const float f = sums.m[w][v] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(sums.m[w][v] - o.m);
     const f32x4 x = *reinterpret_cast<const f32x4*>(&all.acc[w][v][4 * c]);
     o.l += sums.l[w][v] * f;
@@ -569,7 +580,7 @@ template <int G, int FORM>
 __global__ __launch_bounds__(kThreads, 4) void prefix_kernel(Args a, const uint32_t* __restrict__ table, uint32_t stride,
                                                              uint32_t items, float* rec, uint32_t* counters,
                                                              uint32_t ncounters, Groups gs) {
-  __shared__ __attribute__((aligned(16))) unsigned char lds_raw[sizeof(NarrowState)];
+  __shared__ __attribute__((aligned(16))) unsigned char lds_raw[sizeof(NarrowState<kWaves>)];
   const uint32_t h = blockIdx.x % a.kvh, item = blockIdx.x / a.kvh;
   if (blockIdx.x == 0 && threadIdx.x < ncounters) counters[threadIdx.x] = 0u;
   if (item >= items) return;
@@ -584,8 +595,8 @@ __global__ __launch_bounds__(kThreads, 4) void prefix_kernel(Args a, const uint3
   const uint32_t* trow = table + (uint64_t)row0 * stride;
   rec += (((uint64_t)row0 * a.qh + h * G) * gs.prefix_slots + chunk) * kRecord;
   if constexpr (FORM == 0) {
-    __shared__ NarrowSums sums;
-    attend_narrow<G>(lds_raw, sums, a, trow, row0, nrows, key0, key1, h);
+    __shared__ NarrowSums<kWaves> sums;
+    attend_narrow<G, kWaves>(lds_raw, sums, a, trow, row0, nrows, key0, key1, h);
     for (uint32_t idx = threadIdx.x; idx < nrows * G * 32; idx += kThreads) {
       const uint32_t v = idx >> 5, c = idx & 31;
       const Part o = narrow_part(lds_raw, sums, v, c);
@@ -618,19 +629,20 @@ __global__ __launch_bounds__(kThreads, 4) void prefix_kernel(Args a, const uint3
 #if defined(__HIP_DEVICE_COMPILE__) && !defined(__gfx950__)
 #error "k_attention_prefix.hip: the in-kernel merge is written for gfx950's memory-model lowering"
 #endif
-template <int G>
-__global__ __launch_bounds__(kThreads, 4) void own_kernel(Args a, const uint32_t* __restrict__ positions,
+template <int G, int NW>
+__global__ __launch_bounds__(64 * NW, 4) void own_kernel(Args a, const uint32_t* __restrict__ positions,
                                                           const uint32_t* __restrict__ table, uint32_t rows,
                                                           uint32_t stride, uint32_t context, uint32_t max_parts,
                                                           uint32_t part_keys,
                                                           const float* __restrict__ prefix_rec, float* part_rec,
                                                           uint32_t* counters, uint16_t* __restrict__ out,
                                                           uint32_t out_mtiles, Groups gs) {
+  constexpr uint32_t kThreads = 64 * NW, kStep = 32 * NW;
   constexpr uint32_t kDims = G * 32;                // (vector, four dims) pairs
   constexpr uint32_t kTeams = kThreads / kDims;     // threads per pair, for the prefix's records
   constexpr int kInFlight = 4;
-  __shared__ __attribute__((aligned(16))) unsigned char lds_raw[sizeof(NarrowState)];
-  __shared__ NarrowSums sums;
+  __shared__ __attribute__((aligned(16))) unsigned char lds_raw[sizeof(NarrowState<NW>)];
+  __shared__ NarrowSums<NW> sums;
   const uint32_t h = blockIdx.x % a.kvh, r = blockIdx.x / a.kvh % rows, part = blockIdx.x / a.kvh / rows;
   const uint32_t pos = uniform(positions[r]), prefix = prefix_of(gs, r);
   if (pos >= context || pos / 16 >= stride || pos + 1 < prefix) {
@@ -667,7 +679,7 @@ __global__ __launch_bounds__(kThreads, 4) void own_kernel(Args a, const uint32_t
     if (c == 0) team_ml[team][v] = make_float2(t.m, t.l);
   }
   const uint32_t key0 = prefix + part * keys, key1 = min(key0 + keys, pos + 1);
-  attend_narrow<G>(lds_raw, sums, a, table + (uint64_t)r * stride, r, 1, key0, key1, h);
+  attend_narrow<G, NW>(lds_raw, sums, a, table + (uint64_t)r * stride, r, 1, key0, key1, h);
   const bool mine = threadIdx.x < kDims;
   Part o = no_part();
   if (mine) {
@@ -725,21 +737,26 @@ __global__ __launch_bounds__(kThreads, 4) void own_kernel(Args a, const uint32_t
 // that the scratch's size and the launch agree.
 struct PrefixPlan {
   Groups gs;
-  uint32_t items, form, max_parts, part_keys, counters;
+  uint32_t items, form, max_parts, part_keys, own_waves, counters;
   uint64_t prefix_floats, part_floats;  // of the records
 };
 
-PrefixPlan prefix_plan(const fh_prefix_group* groups, uint32_t ngroups, uint32_t rows, uint32_t qh, uint32_t kvh) {
+// (context: an upper bound of the positions, for the own keys' form alone; the scratch does not depend on it.)
+PrefixPlan prefix_plan(const fh_prefix_group* groups, uint32_t ngroups, uint32_t rows, uint32_t qh, uint32_t kvh,
+                       uint32_t context) {
   PrefixPlan p{};
   const uint32_t g = qh / kvh;
-  uint32_t most = 0, longest = 0;
+  uint32_t most = 0, longest = 0, shortest = context, grouped = 0;
   for (uint32_t i = 0; i < ngroups; ++i) {
     if (groups[i].prefix_pages == 0) continue;
     Group& to = p.gs.g[p.gs.count++];
     to = Group{groups[i].first_row, groups[i].rows, groups[i].prefix_pages * 16, 0};
     if (to.rows > most) most = to.rows;
     if (to.prefix_tokens > longest) longest = to.prefix_tokens;
+    if (to.prefix_tokens < shortest) shortest = to.prefix_tokens;
+    grouped += to.rows;
   }
+  if (grouped < rows) shortest = 0;
   const uint64_t vectors = (uint64_t)most * g;
   if (most == 0) most = 1;
   // Tokens times blocks times KV heads with blocks of `rows` rows.
@@ -771,6 +788,7 @@ PrefixPlan prefix_plan(const fh_prefix_group* groups, uint32_t ngroups, uint32_t
   const uint64_t pairs = (uint64_t)rows * kvh;
   p.max_parts = pairs >= kSlots ? 1 : (uint32_t)(kSlots / pairs) < kMaxParts ? (uint32_t)(kSlots / pairs) : kMaxParts;
   p.part_keys = pairs > kManyPairs ? kPartKeysMany : kPartKeysFew;
+  p.own_waves = pairs >= kManyOwn && context - shortest <= kShortOwn ? 4 : 8;
   p.counters = p.max_parts > 1 ? (uint32_t)pairs : 0;
   p.prefix_floats = (uint64_t)rows * qh * p.gs.prefix_slots * kRecord;
   p.part_floats = p.max_parts > 1 ? (uint64_t)rows * qh * p.max_parts * kRecord : 0;
@@ -780,7 +798,7 @@ PrefixPlan prefix_plan(const fh_prefix_group* groups, uint32_t ngroups, uint32_t
 }  // namespace
 
 uint64_t prefix_scratch_bytes(const fh_prefix_group* groups, uint32_t ngroups, uint32_t rows, uint32_t qh, uint32_t kvh) {
-  const PrefixPlan p = prefix_plan(groups, ngroups, rows, qh, kvh);
+  const PrefixPlan p = prefix_plan(groups, ngroups, rows, qh, kvh, 0);
   return (p.prefix_floats + p.part_floats + p.counters + 4) * 4;  // never nothing
 }
 
@@ -789,7 +807,7 @@ hipError_t launch_prefix_attention(const uint16_t* q, const uint16_t* k_cache, c
                                    uint32_t ngroups, uint16_t* out, uint32_t out_tiled, void* scratch, uint32_t rows,
                                    uint32_t qh, uint32_t kvh, uint32_t stride, uint32_t pages, uint32_t context,
                                    uint32_t* err, hipStream_t s) {
-  const PrefixPlan p = prefix_plan(groups, ngroups, rows, qh, kvh);
+  const PrefixPlan p = prefix_plan(groups, ngroups, rows, qh, kvh, context);
   float* prefix_rec = reinterpret_cast<float*>(scratch);
   float* part_rec = prefix_rec + p.prefix_floats;
   uint32_t* counters = reinterpret_cast<uint32_t*>(part_rec + p.part_floats);
@@ -799,6 +817,9 @@ hipError_t launch_prefix_attention(const uint16_t* q, const uint16_t* k_cache, c
 #define FH_PREFIX_FORM(G_, FORM_)                                                                                      \
   hipLaunchKernelGGL((prefix_kernel<G_, FORM_>), dim3(prefix_wgs), dim3(kThreads), 0, s, a, table, stride, p.items, \
                      prefix_rec, counters, p.counters, p.gs)
+#define FH_PREFIX_OWN(G_, NW_)                                                                                      \
+  hipLaunchKernelGGL((own_kernel<G_, NW_>), dim3(kvh * rows * p.max_parts), dim3(64 * NW_), 0, s, a, positions, table, \
+                     rows, stride, context, p.max_parts, p.part_keys, prefix_rec, part_rec, counters, out, mt, p.gs)
 #define FH_PREFIX(G_)                                                                                               \
   do {                                                                                                              \
     if (prefix_wgs) {                                                                                               \
@@ -809,9 +830,10 @@ hipError_t launch_prefix_attention(const uint16_t* q, const uint16_t* k_cache, c
       else                                                                                                          \
         FH_PREFIX_FORM(G_, 0);                                                                                      \
     }                                                                                                               \
-    hipLaunchKernelGGL((own_kernel<G_>), dim3(kvh * rows * p.max_parts), dim3(kThreads), 0, s, a, positions, table, \
-                       rows, stride, context, p.max_parts, p.part_keys, prefix_rec, part_rec, counters, out, mt,    \
-                       p.gs);                                                                                       \
+    if (p.own_waves == 4)                                                                                           \
+      FH_PREFIX_OWN(G_, 4);                                                                                         \
+    else                                                                                                            \
+      FH_PREFIX_OWN(G_, 8);                                                                                         \
   } while (0)
   switch (qh / kvh) {
     case 1: FH_PREFIX(1); break;
@@ -822,6 +844,7 @@ hipError_t launch_prefix_attention(const uint16_t* q, const uint16_t* k_cache, c
   }
 #undef FH_PREFIX
 #undef FH_PREFIX_FORM
+#undef FH_PREFIX_OWN
   return hipGetLastError();
 }
 

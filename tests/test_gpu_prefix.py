@@ -229,6 +229,18 @@ def test_a_run_with_a_position_or_page_out_of_range_in_its_midst():
     holds(b, bits, range(7))
 
 
+@pytest.mark.parametrize("heads", [(32, 8), (16, 8), (8, 8), (64, 8)])
+@pytest.mark.parametrize("longest", [1, 127, 128, 129, 300, 520])
+def test_many_rows_with_short_and_longer_own_keys(longest, heads):
+    """Own keys around the steps of both forms of workgroup, and a context that bounds them and one that does not."""
+    owns = [longest - (i * 7) % longest for i in range(66)]
+    b = Batch(longest, [(owns, 5), ([longest, 1], 7)], *heads, extra_stride=40).device()
+    for context in (int(b.lengths.max()), b.context):
+        bits, err = b.run(context=context)
+        assert err == 0
+        holds(b, bits)
+
+
 def test_sixty_four_groups_of_one_row_and_empty_ones():
     b = Batch(1, [([1 + i % 40], 1 + i % 3) for i in range(64)], 16, 8).device()
     bits, err = b.run()
