@@ -27,7 +27,7 @@
 // last row again (less to fetch; their output rows are not stored).
 //
 // What bounds it: the weights' bytes from HBM in 7 rows through 151936 x 4096 (60
-// us, 325 MB at 5.4 TB/s, the rate of a large copy); a launch's start and end beside them
+// us, 345 MB at 5.7 TB/s; a large copy reaches 5.4, reads alone 6.0); a launch's start and end beside them
 // in one row through 24576 x 4096 (11.9 us, 52 MB; 9.6 at that rate). From about 16
 // rows on, and with few weight rows a workgroup, the activations, which every workgroup
 // reads whole from the L2: 32 rows through 4096 x 12288 take 786 KB into each CU
