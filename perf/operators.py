@@ -74,8 +74,11 @@ def draw(rng):
                     lo=max(per, hi // rng.choice([2, 8, 1000])), hi=hi, per=per)
     n, k = rng.choice([(6144, 4096), (4096, 4096), (24576, 4096), (4096, 12288), (4096, 1024), (1024, 2048),
                        (6144, 1024), (32 * _log(rng, 1, 1000), 128 * _log(rng, 1, 64)), (151936, rng.choice([1024, 4096]))])
-    return dict(kind=kind, n=n, k=k, m=_log(rng, 1, 32), group=rng.choice([32, 64, 128, 128]),
+    case = dict(kind=kind, n=n, k=k, m=_log(rng, 1, 32), group=rng.choice([32, 64, 128, 128]),
                 zeros=rng.choice([0, 1]), epilogue="f32" if n == 151936 else rng.choice(["bf16", "swiglu", "f32"]))
+    if case["epilogue"] == "swiglu":  # the next projection's operand comes in whole blocks of 32 columns
+        case["n"] += n % 64
+    return case
 
 
 # ---- inputs ---------------------------------------------------------------
@@ -189,7 +192,7 @@ def prepare(case, seed):
                  zeros_tiled=_tile_rows(lay(zeros), n) if zeros is not None else None,
                  error=torch.zeros(1, dtype=torch.int32, device="cuda"))
     if wide:  # the next projection's operand: 32 rows in tile order, those past m as they were
-        state["out"] = torch.zeros((n // 64, 2, 4, 16, 8), dtype=torch.bfloat16, device="cuda")
+        state["out"] = torch.zeros((-(-n // 64), 2, 4, 16, 8), dtype=torch.bfloat16, device="cuda")
     else:
         state["out"] = torch.empty((m, n), dtype=torch.float32 if case["epilogue"] == "f32" else torch.bfloat16,
                                    device="cuda")
