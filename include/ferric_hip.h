@@ -286,7 +286,8 @@ fh_status fh_op_rmsnorm(const uint16_t* x, const uint16_t* weight, uint16_t* y, 
  * activation.rs:32 and device/qwen3-tp-fp32-head32-kernels-v8/src/projection.rs:66/:186. */
 enum { FH_EPI_BF16 = 0, FH_EPI_RESIDUAL = 1, FH_EPI_SWIGLU = 2, FH_EPI_F32 = 3, FH_EPI_PARTIAL = 4 };
 /* x_tiled is in activation tile order (fh_op_tile_activation). FH_EPI_SWIGLU writes its
- * output in activation tile order (the down projection's input); FH_EPI_PARTIAL writes
+ * output in activation tile order (the down projection's input: fh_activation_rows(m) rows of
+ * n / 2 columns rounded up to a multiple of 32); FH_EPI_PARTIAL writes
  * FP32 partial sums as `splits` slabs of [fh_partial_slab_rows(m)][ldo] (split-K across
  * workgroups; the consumer adds the slabs in order and rounds once; a split past the end
  * of k writes zeros). Other epilogues use splits = 1.
@@ -302,9 +303,11 @@ fh_status fh_op_gemm(const uint16_t* x_tiled, const uint16_t* w_tiled, uint32_t 
  * than 2^122 in a group, or that holds an infinity, may give NaN). n % 16 == 0 (32 for
  * FH_EPI_SWIGLU), k % 128 == 0, k <= 2^24, n * k < 2^35, group 32, 64 or 128. Epilogues,
  * x_tiled, splits (<= k / 128 and 65535), residual, out, ldo and error_word as fh_op_gemm; only
- * the first m rows of out are written. Operands in the order fh_op_tile_weight_w4 writes, w_tiled and x_tiled 16-byte, scales_tiled 8-byte and
- * zeros_tiled 4-byte aligned. No counterpart in the reference, whose projections read bf16
- * weights (gemm.rs:161/:605). */
+ * the first m rows of out are written. FH_EPI_SWIGLU's out holds whole blocks of 32 rows x 32
+ * columns, 1024 x ceil(n / 64) elements: where n / 2 is no multiple of 32, the last block's other
+ * 16 columns keep their values. Operands in the order fh_op_tile_weight_w4 writes, w_tiled and
+ * x_tiled 16-byte, scales_tiled 8-byte and zeros_tiled 4-byte aligned. No counterpart in the
+ * reference, whose projections read bf16 weights (gemm.rs:161/:605). */
 fh_status fh_op_gemm_w4(const uint16_t* x_tiled, const uint32_t* w_tiled, const uint16_t* scales_tiled,
                         const uint8_t* zeros_tiled, uint32_t m, uint32_t n, uint32_t k, uint32_t group,
                         uint32_t epilogue, uint32_t splits, const uint16_t* residual, void* out, uint32_t ldo,

@@ -214,6 +214,32 @@ def test_swiglu_reports_nonfinite_rows_below_m_only():
     assert du.to_host(err, np.uint32)[0] == 1
 
 
+@pytest.mark.parametrize("width", [16, 48, 80])
+@pytest.mark.parametrize("m", [1, 17])
+def test_swiglu_of_half_a_block_of_columns_stays_in_its_blocks(width, m):
+    """n / 2 an odd multiple of 16: out holds ceil(n / 64) blocks of 32 x 32, nothing behind them or in the last
+    block's other columns is written."""
+    r = np.random.default_rng(width + m)
+    gate = Weight(r, width, 128, 64, True, half=True)
+    up = Weight(r, width, 128, 64, True, half=True)
+    gate.tile(gate, 1)
+    up.tile(gate, 2)
+    x, xt = activations(r, m, 128, whole=True)
+    blocks = -(-width // 32)
+    out = du.to_dev(np.full(1024 * blocks + 1024, 0x2222, np.uint16))
+    call(xt, gate, m, 2 * width, SWIGLU, out, width)
+    got = du.to_host(out, np.uint16)
+    assert np.all(got[1024 * blocks:] == 0x2222)
+    tiled = got[:1024 * blocks].reshape(blocks, 2, 4, 16, 8).transpose(1, 3, 0, 2, 4).reshape(32, 32 * blocks)
+    assert np.all(tiled[m:] == 0x2222) and np.all(tiled[:, width:] == 0x2222)
+    # Exact sums narrowed to bf16; the exponential, a quotient and two products round in FP32, together less than
+    # 2^-20, then half a step of bf16 (results below the normal numbers, 2^-126, aside).
+    g, u = (widen(narrow(widen(x) @ w.exact().T)) for w in (gate, up))
+    with np.errstate(over="ignore"):
+        want = g / (1 + np.exp(-g)) * u
+    assert np.all(np.abs(widen(tiled[:m, :width]) - want) <= (2.0 ** -8 + 2.0 ** -20) * np.abs(want) + 1e-30)
+
+
 def test_extremes_of_weights_and_scales():
     """All weights at the ends, scales at the ends of bf16, zero scales, zero points 0 and 15."""
     r = np.random.default_rng(1)

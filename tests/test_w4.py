@@ -1,7 +1,10 @@
 """4-bit projections on any host: what the entry points refuse before any
 launch. No GPU calls are made here (the pointers are no memory)."""
 
+import importlib.util
 import itertools
+import random
+from pathlib import Path
 
 import pytest
 
@@ -47,3 +50,14 @@ def test_default_splits_fill_the_gpu_and_fit_the_width():
     assert LIB.fh_gemm_w4_default_splits(4096, 4096) == 2
     assert LIB.fh_gemm_w4_default_splits(24576, 4096) == 1
     assert LIB.fh_gemm_w4_default_splits(0, 4096) == 1
+
+
+def test_measured_swiglu_cases_have_whole_blocks_of_output_columns():
+    """Their outputs are the next projection's operand, whose buffers are cut to blocks of 32 columns."""
+    spec = importlib.util.spec_from_file_location("operators", Path(__file__).resolve().parents[1] / "perf" / "operators.py")
+    operators = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(operators)
+    cases = operators.listed() + [operators.draw(random.Random(s)) for s in range(4000)]
+    wide = [c for c in cases if c.get("epilogue") == "swiglu"]
+    assert len(wide) > 100
+    assert all(c["n"] % 64 == 0 for c in wide)
