@@ -317,3 +317,86 @@ def test_two_streams_and_a_replayed_graph():
         torch.cuda.synchronize()
         for o in outs:
             assert np.array_equal(du.to_host(o, np.float32).reshape(m, n), want)
+
+
+# ---- every form of workgroup -------------------------------------------------------
+
+def on_device(w):
+    """W in 64 bits on the device, [n][k]."""
+    rep = lambda a: a.repeat_interleave(w.group, 1)  # noqa: E731
+    s = torch.from_numpy(widen(w.s)).cuda()
+    z = torch.from_numpy(w.z).cuda().double() if w.z is not None else torch.full_like(s, 8.0)
+    return rep(s) * (torch.from_numpy(w.q).cuda().double() - rep(z))
+
+
+def product(x, w):
+    return (torch.from_numpy(widen(x)).cuda() @ on_device(w).t()).cpu().numpy()
+
+
+# Both sides of the sizes from which workgroups have 2 and 4 weight tiles and 4 waves instead of 16, an odd number of
+# 32-column pairs, and widths whose blocks of 128 columns the waves take in several turns, the last one short.
+FORMS = [(8192, 4224, (1, 8, 16, 17, 32)), (8208, 1152, (1, 16, 17, 32)), (16368, 1152, (2, 18)),
+         (16384, 1152, (1, 8, 9, 16, 17, 32)), (16416, 1152, (8, 9, 17, 32)), (65536, 640, (1, 8, 9, 32)),
+         (65568, 640, (1, 9, 32)), (4096, 6528, (16, 17, 32))]
+
+
+@pytest.mark.parametrize("n,k,rows", FORMS)
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_every_form_is_exact_on_whole_numbers(n, k, rows, group, zeros):
+    r = np.random.default_rng(n + group)
+    w = Weight(r, n, k, group, zeros)
+    for m in rows:
+        x, xt = activations(r, m, k, whole=True)
+        want = product(x, w)
+        out = torch.full(((m + 1) * n,), 7.5, dtype=torch.float32, device="cuda")
+        call(xt, w, m, n, F32, out, n)
+        got = du.to_host(out, np.float32).reshape(m + 1, n)
+        assert np.array_equal(got[:m], want) and np.all(got[m] == 7.5), m
+        res = orc.f32_to_bf16(r.integers(-99, 99, m * n).astype(np.float32))
+        dres, out = du.to_dev(res), du.to_dev(np.full((m + 1) * n, 0x1234, np.uint16))
+        call(xt, w, m, n, RESIDUAL, out, n, residual=dres)
+        got = du.to_host(out, np.uint16).reshape(m + 1, n)
+        assert np.array_equal(got[:m], narrow(want + widen(res).reshape(m, n))) and np.all(got[m] == 0x1234), m
+
+
+@pytest.mark.parametrize("n", [4096, 4112])
+@pytest.mark.parametrize("m", [1, 9, 32])
+@pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, True)])
+def test_split_slabs_of_wide_weights_add_up_exactly(n, m, group, zeros):
+    r = np.random.default_rng(n + m)
+    k, splits = 2176, 4  # 17 blocks of 128 columns: 5, 5, 5 and 2
+    w = Weight(r, n, k, group, zeros)
+    x, xt = activations(r, m, k, whole=True)
+    out = torch.full(((splits * 32 + 1) * n,), 7.5, dtype=torch.float32, device="cuda")
+    call(xt, w, m, n, PARTIAL, out, n, splits)
+    got = du.to_host(out, np.float32).reshape(-1, n)
+    slabs = got[:splits * 32].reshape(splits, 32, n)
+    assert np.array_equal(slabs[:, :m].astype(np.float64).sum(0), product(x, w))
+    assert np.all(slabs[:, m:] == 7.5) and np.all(got[-1] == 7.5)
+
+
+@pytest.mark.parametrize("n,m", [(8192, 17), (16352, 1), (16384, 1), (16384, 9), (16384, 17), (16416, 32), (24576, 1),
+                                 (24576, 32), (65536, 1), (65536, 8)])
+@pytest.mark.parametrize("group,zeros", [(32, True), (64, True), (128, False)])
+def test_swiglu_of_every_form(n, m, group, zeros):
+    """Exact sums (scales are powers of two) narrowed to bf16; the exponential, a quotient and two products round in
+    FP32, together less than 2^-20, then half a step of bf16."""
+    r = np.random.default_rng(n + m)
+    width, k = n // 2, 640
+    scale = lambda: orc.f32_to_bf16((2.0 ** r.integers(-9, -6, width * (k // group))).astype(np.float32))  # noqa: E731
+    gate = Weight(r, width, k, group, zeros, scales=scale(), half=True)
+    up = Weight(r, width, k, group, zeros, scales=scale(), half=True)
+    gate.tile(gate, 1)
+    up.tile(gate, 2)
+    x, xt = activations(r, m, k, whole=True)
+    blocks = -(-width // 32)
+    out, err = du.to_dev(np.full(1024 * blocks + 1024, 0x2222, np.uint16)), du.empty(1, np.uint32)
+    call(xt, gate, m, n, SWIGLU, out, width, err=err)
+    assert du.to_host(err, np.uint32)[0] == 0
+    got = du.to_host(out, np.uint16)
+    tiled = got[:1024 * blocks].reshape(blocks, 2, 4, 16, 8).transpose(1, 3, 0, 2, 4).reshape(32, 32 * blocks)
+    assert np.all(got[1024 * blocks:] == 0x2222) and np.all(tiled[m:] == 0x2222) and np.all(tiled[:, width:] == 0x2222)
+    g, u = (widen(narrow(product(x, w))) for w in (gate, up))
+    want = g / (1 + np.exp(-g)) * u
+    assert np.all(np.abs(widen(tiled[:m, :width]) - want) <= (2.0 ** -8 + 2.0 ** -20) * np.abs(want) + 1e-30)
