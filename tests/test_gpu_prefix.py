@@ -483,3 +483,72 @@ def test_fork_then_shared_attention_then_a_4_bit_projection():
     # The products' FP32 error, 1e-5 of the result's norm if independent, and the weight's rounding to 4 bits.
     assert np.linalg.norm(y.cpu().numpy() - want) <= 2e-5 * np.linalg.norm(want)
     assert np.all(np.abs((q * s).reshape(n, k) - w) <= np.repeat(s[..., 0], group, 1) * 0.52 + 2.0 ** -8 * np.abs(w))
+
+
+# ---- long prefixes: chunks of many tiles, blocks of 128 vectors, streamed loads -----
+
+class Long(Batch):
+    """The formula on the device, and values that mark the keys: with queries of zero every key has the same weight,
+    and key t is 1 in one (KV head, dim) of 1024 and 0 elsewhere, so a key more or less changes an output by one part
+    in about n / 1024."""
+
+    def exact(self, rows=None):
+        g = self.qh // self.kvh
+        want = torch.zeros(self.rows, self.qh, 128, dtype=torch.float64)
+        tol = torch.zeros_like(want)
+        for r in range(self.rows) if rows is None else rows:
+            n = int(self.lengths[r])
+            idx = torch.from_numpy(self.table[r, :-(-n // 16)].astype(np.int64)).cuda()
+            k = self.d["k"][idx].view(-1, self.kvh, 128)[:n].double().permute(1, 2, 0).contiguous()  # [kvh][128][n]
+            v = self.d["v"][idx].view(-1, self.kvh, 128)[:n].double().permute(1, 0, 2).contiguous()
+            q = self.d["q"][r].double().view(self.kvh, g, 128)
+            s = torch.matmul(q, k) / math.sqrt(128)
+            most = torch.matmul(q.abs(), k.abs()).amax((1, 2)).view(-1, 1, 1) / math.sqrt(128)
+            w = torch.softmax(s, -1)
+            want[r] = torch.matmul(w, v).view(self.qh, 128).cpu()
+            d = 128 * 2.0 ** -24 * most + 2.0 ** -22 + 2.0 ** -23 * s.abs().amax()
+            tol[r] = (torch.matmul(w, v.abs()) * (2 * d + 2.0 ** -16 + n * 2.0 ** -24)).view(self.qh, 128).cpu()
+        return want, tol + 2.0 ** -8 * (want.abs() + tol)
+
+    def mark(self):
+        assert self.kvh == 8
+        self.d["q"].zero_()
+        ones = torch.eye(1024, dtype=torch.bfloat16, device="cuda").view(1024, 8, 128)
+        for r in range(self.rows):
+            t = torch.arange(int(self.lengths[r]), device="cuda")
+            page = torch.from_numpy(self.table[r].astype(np.int64)).cuda()[t // 16]
+            self.d["v"][page, t % 16] = ones[t % 1024]
+
+    def marked(self):
+        """(output, tolerance) of the marked values: keys of a bin over all keys; the scores are 0 exactly."""
+        n = torch.from_numpy(self.lengths.astype(np.float64)).view(-1, 1, 1)
+        bins = torch.arange(1024, dtype=torch.float64).view(1, 8, 128)
+        want = (torch.floor((n - 1 - bins) / 1024) + 1) / n
+        want = want.repeat_interleave(self.qh // self.kvh, 1)
+        tol = want * (2.0 ** -21 + 2.0 ** -16 + n * 2.0 ** -24)
+        return want, tol + 2.0 ** -8 * (want + tol)
+
+
+@pytest.mark.parametrize("heads", [(8, 8), (16, 8), (32, 8), (64, 8)])
+@pytest.mark.parametrize("vectors", [16, 40, 64, 72, 128, 136])
+@pytest.mark.parametrize("pages", [1030, 1541])
+def test_long_prefixes(heads, vectors, pages):
+    """One and several blocks of 16, 64 and 128 vectors, part of them filled; the longer prefix is streamed where one
+    block holds the rows."""
+    rows = vectors // (heads[0] // heads[1])
+    groups = [([i * 5 % 23 for i in range(rows)], pages)] + ([([5, 1], 2), ([9], 0)] if vectors == 40 else [])
+    b = Long(vectors + pages, groups, *heads).device()
+    bits, err = b.run()
+    assert err == 0
+    holds(b, bits, sorted({0, rows // 2, rows - 1, b.rows - 1}))
+    again, _ = b.run()
+    assert np.array_equal(bits, again)
+    b.mark()
+    bits, err = b.run()
+    assert err == 0
+    want, tol = b.marked()
+    off = (values(bits, b) - want).abs()
+    assert bool((off <= tol).all()), float((off / tol).max())
+    # One key less would be seen: the largest bin's output falls by more than twice its tolerance.
+    n = int(b.lengths[0])
+    assert (1 / n) > 2 * float(tol[0].max())
