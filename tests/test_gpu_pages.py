@@ -164,3 +164,22 @@ def test_moves_reach_every_layer_of_k_and_v_and_no_other_page():
                 assert np.array_equal(runner.read_kv_cache(l, w), content[l, w].reshape(-1))
     finally:
         runner.close()
+
+
+@pytest.mark.parametrize("count", [255, 700])
+def test_calls_of_more_than_the_caches_hold(count):
+    """From 256 MB on the copies stream past the caches: one launch and several, whole pages and parts of them."""
+    r = np.random.default_rng(count)
+    kvh, caches, pages = 8, 72, 1500
+    moves = moves_of(r, pages, count, 16 if count < 256 else None)
+    assert int(moves[:, 2].sum()) * kvh * 256 * caches >= 1 << 28
+    g = torch.Generator(device="cuda").manual_seed(count)
+    dev = torch.empty(caches, pages, 16, kvh * 128, dtype=torch.int16, device="cuda").random_(-32768, 32768, generator=g)
+    want = dev.clone()
+    src, dst, n = (torch.from_numpy(moves[:, i].astype(np.int64)).cuda() for i in range(3))
+    kept = (torch.arange(16, device="cuda")[None, :] < n[:, None])[:, :, None]
+    for c in range(caches):  # no destination is a source or occurs twice
+        want[c, dst] = torch.where(kept, want[c, src], want[c, dst])
+    call(dev, caches, pages * 16 * kvh * 128, moves, kvh, pages)
+    torch.cuda.synchronize()
+    assert torch.equal(dev, want)
