@@ -120,6 +120,7 @@ SIGNATURES = [
     ("fh_kv_copy_pages", _st, [_vp, _vp, _u32]),
     ("fh_execute_batch", _st, [_vp, _u64, ctypes.POINTER(Row), _u32, _u32p, _u32, _u32p]),
     ("fh_execute_batch_shared", _st, [_vp, _u64, ctypes.POINTER(Row), _u32, _vp, _u32, _u32p, _u32, _u32p]),
+    ("fh_prefix_groups_gain", _u32, [_vp] + [_u32] * 4),
     ("fh_read_logits", _st, [_vp, _f32p, _u64]),
     ("fh_read_hidden", _st, [_vp, _u32, _u16p, _u64]),
     ("fh_row_capacity", _u32, [_vp]),

@@ -417,6 +417,23 @@ uint64_t fh_prefix_attention_scratch_bytes(const fh_prefix_group* groups, uint32
   return fh::prefix_scratch_bytes(groups, ngroups, rows, query_heads, kv_heads);
 }
 
+uint32_t fh_prefix_groups_gain(const fh_prefix_group* groups, uint32_t ngroups, uint32_t rows, uint32_t kv_heads,
+                               uint32_t context_tokens) {
+  if (ngroups == 0 || kv_heads == 0 || rows == 0 || context_tokens == 0 ||
+      fh::prefix_groups_refused(groups, ngroups, rows, context_tokens))
+    return 0;
+  // What sharing saves a layer, in keys of one head: those that the rows of a group after its first do not read
+  // again, and a workgroup of the rows' own attention per 512 tokens of the context, the idle ones too, worth
+  // about 34 keys. It costs two more launches and the QK-norm outside the attention, worth 140000. Fitted to steps
+  // of 2 to 32 rows behind 16 to 32000 tokens in contexts of 1280 to 33024, of Qwen3-0.6B and Qwen3-8B shapes: where
+  // this says 1 the worst is 0.5 % slower than unshared, where it says 0 the best would have been 8 % faster (with
+  // 131072: 3.9 and 8; with every group shared, 31 % slower at worst).
+  constexpr uint64_t kPartition = 34, kLaunches = 140000;
+  uint64_t saved = kPartition * ((context_tokens - 1) / 512 + 1) * rows;
+  for (uint32_t i = 0; i < ngroups; ++i) saved += (uint64_t)(groups[i].rows - 1) * groups[i].prefix_pages * 16;
+  return saved >= (kLaunches + kv_heads - 1) / kv_heads ? 1 : 0;
+}
+
 fh_status fh_op_prefix_attention(const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache,
                                  const uint32_t* positions, const uint32_t* page_table,
                                  const fh_prefix_group* groups, uint32_t ngroups, uint16_t* out, uint32_t out_tiled,

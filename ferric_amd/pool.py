@@ -316,11 +316,9 @@ class PagePool:
         """Runs of consecutive rows of a decode batch that list the same pages
         first, as TpBatchRunner.execute_batch takes them: [(first row, rows, prefix
         pages)]. Only whole pages before every row's written one count. A run goes
-        on while the page reads saved, (rows - 1) * pages, do not fall. Sharing
-        gains from about 8 rows on at any length (device time of a step, Qwen3-8B
-        shape, one prompt: 32 rows behind 8192 tokens 11.39 -> 4.25 ms, behind 64
-        4.22 -> 3.80), with fewer rows from about 1000 tokens (4 rows: 3.58 -> 3.46
-        ms; behind 64 tokens 3.37 -> 3.43); min_pages leaves shorter ones out."""
+        on while the page reads saved, (rows - 1) * pages, do not fall. min_pages
+        leaves shorter prefixes out. All runs are returned, also those whose step is
+        faster unshared: TpBatchRunner.gaining_groups decides that for the step."""
         lists = [(np.asarray(r.physical_pages), r.position // PAGE_TOKENS) for r in batch.rows]
         groups, i = [], 0
         while i < len(lists):

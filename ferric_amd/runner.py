@@ -246,7 +246,8 @@ class TpBatchRunner:
     def execute_batch(self, batch: PreparedBatch, output_rows: Sequence[int], prefix_groups=()) -> BatchOutput:
         """One step. prefix_groups: [(first row, rows, prefix pages)] of a decode
         batch whose rows share prefixes (PagePool.prefix_groups), whose pages
-        the attention then reads once a group (fh_execute_batch_shared)."""
+        the attention then reads once a group (fh_execute_batch_shared). That is
+        slower for few rows or short prefixes: gaining_groups leaves those out."""
         if batch.limits != self.limits:
             raise FerricError(2, "foreign, stale, or invalid prepared GPU batch")
         rows, keep = _rows_to_c(batch.rows)
@@ -266,6 +267,14 @@ class TpBatchRunner:
         self._rows_last = len(batch.rows) if len(batch.rows) <= self._opts.row_capacity else len(outs)
         self._batch_rows_last = len(batch.rows)
         return BatchOutput([int(c) for c in choices[: len(outs)]])
+
+    def gaining_groups(self, batch: PreparedBatch, prefix_groups) -> list:
+        """The groups of a decode batch if its step is expected to be faster
+        with them than without (fh_prefix_groups_gain), else none."""
+        groups = _groups_to_c(prefix_groups)
+        gain = self._lib.fh_prefix_groups_gain(groups.ctypes.data, len(groups), len(batch.rows), self.model["kv_heads"],
+                                               self.limits.context_tokens)
+        return [tuple(g) for g in groups.tolist()] if gain else []
 
     def output_head_rows(self, physical: int, published: int) -> int:
         return physical

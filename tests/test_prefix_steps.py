@@ -8,7 +8,7 @@ import pytest
 
 import ferric_amd
 from ferric_amd.pool import PagePool
-from ferric_amd.runner import PagedLimits, _groups_to_c
+from ferric_amd.runner import PagedLimits, TpBatchRunner, _groups_to_c
 
 LIB = ferric_amd.load()
 LIMITS = PagedLimits(context_tokens=640, physical_page_count=400, page_table_stride=40)
@@ -92,3 +92,41 @@ def test_no_context():
     assert LIB.fh_execute_batch_shared(None, 1, None, 1, None, 0, None, 0, None) == 1
     n = ctypes.c_uint64()
     assert LIB.fh_expected_dispatch_count_shared(None, 1, None, 1, g.ctypes.data, 1, None, 0, ctypes.byref(n)) == 1
+
+
+@pytest.mark.parametrize("rows,prefix,context,gains", [
+    # Measured steps of Qwen3-0.6B and Qwen3-8B shapes, shared against not: slower in both, or faster in both.
+    (2, 16, 1280, 0), (8, 64, 1280, 0), (16, 256, 1280, 0), (32, 256, 1280, 0), (32, 1024, 1280, 1), (8, 256, 4352, 0),
+    (16, 1024, 4352, 1), (2, 64, 33024, 0), (4, 64, 33024, 0), (16, 16, 33024, 1), (32, 16, 33024, 1), (4, 4096, 33024, 1),
+    (2, 32000, 33024, 1), (32, 32000, 33024, 1)])
+def test_groups_that_gain(rows, prefix, context, gains):
+    class Runner(TpBatchRunner):
+        def __init__(self):
+            self._lib, self.model = LIB, ferric_amd.QWEN3_8B
+            self.limits = PagedLimits(context, context // 16 + 300, context // 16)
+
+    runner = Runner()
+    pool = PagePool(runner.limits, seed=1)
+    live = [pool.admit(prefix + 5)]
+    live += [pool.fork(live[0])[0] for _ in range(rows - 1)]
+    batch = pool.prepare([(s, 1) for s in live])
+    groups = PagePool.prefix_groups(batch)
+    assert groups == [(0, rows, prefix // 16)]
+    assert runner.gaining_groups(batch, groups) == (groups if gains else [])
+    assert runner.gaining_groups(batch, []) == []
+
+
+def test_gains_of_several_groups_add_up_and_refused_groups_have_none():
+    def gain(groups, rows, heads=8, context=16384):
+        g = np.array(groups, np.uint32).reshape(-1, 3)
+        return LIB.fh_prefix_groups_gain(g.ctypes.data, len(g), rows, heads, context)
+
+    # Of 140000: 34 * 8 rows * 8 heads * 32 parts of the context = 69632; 3 rows * 256 pages * 16 * 8 heads = 98304.
+    assert gain([(0, 4, 256)], 8) == 1 and gain([(4, 4, 256)], 8) == 1 and gain([(0, 4, 256), (4, 4, 256)], 8) == 1
+    assert gain([(0, 4, 128)], 8) == 0 and gain([(4, 4, 128)], 8) == 0 and gain([(0, 4, 128), (4, 4, 128)], 8) == 1
+    assert gain([(0, 4, 128)], 8, heads=16) == 1  # heads count as keys do
+    assert gain([], 32) == 0 and gain([(0, 32, 900)], 32) == 1
+    for bad in ([(0, 33, 900)], [(0, 0, 900)], [(0, 32, 1025)], [(8, 8, 900), (0, 8, 900)]):
+        assert gain(bad, 32) == 0
+    assert gain([(0, 32, 900)], 0) == 0 and gain([(0, 32, 900)], 32, heads=0) == 0 and gain([(0, 32, 0)], 32, context=0) == 0
+    assert LIB.fh_prefix_groups_gain(None, 1, 32, 8, 16384) == 0
