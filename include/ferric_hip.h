@@ -186,7 +186,7 @@ typedef struct fh_prefix_group {
 /* fh_execute_batch for a decode batch (nrows <= row_capacity) whose rows share prefixes
  * (continuations of one prompt): the attention reads the pages of a group's prefix once for
  * its rows (fh_op_prefix_attention) instead of once a row; the logits differ from
- * fh_execute_batch's by the order of sums only. groups: as fh_op_prefix_attention, each with
+ * fh_execute_batch's by that attention's roundings. groups: as fh_op_prefix_attention, each with
  * prefix_pages >= 1 whole pages that every row of it lists at the start of its list and
  * writes behind; else FH_ERR_INVALID_ARGUMENT, and nothing has run. ngroups 0:
  * fh_execute_batch itself. A second step with the same rows and groups is captured into a
@@ -454,15 +454,19 @@ fh_status fh_op_paged_attention_noalloc(const uint16_t* q, const uint16_t* k_cac
  * other keys once for the row. groups is host memory, read before the call returns (a
  * captured graph keeps them): 0..64 groups, ascending and disjoint; rows in no group share
  * nothing. Up to 65535 rows (2^22 with their KV heads) and 2^24 context tokens; several rows may
- * belong to one sequence. Every row of a group has position >= 16 x prefix_pages - 1 (its prefix is all visible; ERR_POSITION in error_word
- * and no output for the row otherwise), and its table's first prefix_pages entries are those
- * of the group's first row (the page bit of error_word otherwise). q, out, out_tiled, tables
+ * belong to one sequence. Every row of a group has position >= 16 x prefix_pages - 1 (its prefix
+ * is all visible; the position bit of error_word and no output for the row otherwise), and its
+ * table's first prefix_pages entries are those of the group's first row (the page bit of
+ * error_word otherwise). q, out, out_tiled, tables
  * and errors as fh_op_paged_attention; q and the caches 16-byte, out 8-byte aligned. scratch:
  * fh_prefix_attention_scratch_bytes() of the same arguments, 16-byte aligned, for this call
- * alone until it has run. Rows with one or several query heads per KV head (1, 2, 4, 8). FP32
- * reassociation: the states of chunks of keys are merged, so the result differs from
- * fh_op_paged_attention's in the order of its sums. No counterpart in the reference, whose
- * decode attention reads every row's context (paged_decode.rs:222). */
+ * alone until it has run. Rows with one or several query heads per KV head (1, 2, 4, 8). The
+ * result differs from fh_op_paged_attention's by two roundings before the last one to bf16: the
+ * states of chunks of keys are merged (FP32 sums in another order), and a probability enters the
+ * product with the values as two bf16 terms, within 2^-17 of it (there as FP32). After the last
+ * one, 1 to 2 elements in 1000 are one bf16 step apart, and both are off by 1.65e-3 of the
+ * output's norm (4 to 160 rows behind 1488 to 32000 tokens). No counterpart in the reference,
+ * whose decode attention reads every row's context (paged_decode.rs:222). */
 uint64_t fh_prefix_attention_scratch_bytes(const fh_prefix_group* groups, uint32_t ngroups, uint32_t rows,
                                            uint32_t query_heads, uint32_t kv_heads, uint32_t context_tokens);
 fh_status fh_op_prefix_attention(const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache,
