@@ -189,9 +189,11 @@ typedef struct fh_prefix_group {
  * fh_execute_batch's by that attention's roundings. groups: as fh_op_prefix_attention, each with
  * prefix_pages >= 1 whole pages that every row of it lists at the start of its list and
  * writes behind; else FH_ERR_INVALID_ARGUMENT, and nothing has run. ngroups 0:
- * fh_execute_batch itself. A second step with the same rows and groups is captured into a
- * graph, later ones replay it. The scratch is the context's and grows on demand
- * (FH_ERR_OUT_OF_MEMORY, nothing has run). No counterpart in the reference. */
+ * fh_execute_batch itself. A step with the number of rows and the groups of the shared step
+ * before it is captured into a graph, the next such steps replay it; there is one such graph,
+ * so shared steps that alternate between two batches launch their kernels one by one
+ * (Qwen3-0.6B: 0.03 to 0.13 ms a step more, Qwen3-8B: none). The scratch is the context's and
+ * grows on demand (FH_ERR_OUT_OF_MEMORY, nothing has run). No counterpart in the reference. */
 fh_status fh_execute_batch_shared(fh_ctx* ctx, uint64_t batch_id, const fh_row* rows, uint32_t nrows,
                                   const fh_prefix_group* groups, uint32_t ngroups, const uint32_t* output_rows,
                                   uint32_t nout, uint32_t* choices_out);
