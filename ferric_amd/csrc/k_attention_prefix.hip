@@ -38,18 +38,20 @@
 // the next fetch. Narrow (own keys, and prefix chunks of up to 16 vectors): the waves
 // take 32 keys each, K straight into the A operand's registers (a token's 64-byte
 // pieces), V through 8 KiB of LDS of the wave's own; their states meet in LDS at the
-// end. All forms keep to 128 registers a thread and 67.6 KB of LDS (own keys in
-// workgroups of 4 waves to half of it), so that two workgroups (four) share a CU and
-// one computes while the other waits.
+// end. All forms keep to 128 registers a thread, and to 68.6 KB of LDS for a prefix's
+// chunks and 76.9 KB (in workgroups of 4 waves 38.5) for own keys, so that two
+// workgroups (four) can share a CU. Own keys are cut for that many. A long prefix is cut
+// into about as many chunks as there are CUs (kChunkWgs), so there a CU has one
+// workgroup, and its waves have only one another to wait with.
 //
 // What bounds it (kernel times, 32 rows, 8 KV heads of 4 query heads): behind 8192
 // shared tokens the first launch takes 15 us (33.6 MB of keys and values, which the
 // 256 MB cache keeps between steps, and 17 MB of records) and the second 12, a
 // chain of latencies: position -> records -> page table -> keys -> join. Behind
-// 32000 tokens the first takes 38: 131 MB from HBM at 3.5 TB/s, from the bytes that
-// two tiles a workgroup keep in flight. One workgroup a CU with four tiles in flight
-// was slower (18 us and 42): its waves then wait for one another at every tile with
-// nothing else on the CU.
+// 32000 tokens the first takes 38: 131 MB from HBM at 3.5 TB/s, a tile of 32 KB a CU
+// in flight while the one before is computed, which takes turns with the loads at a
+// barrier each tile. Four tiles in flight were slower (18 us and 42), for a reason
+// that was not found.
 #include <type_traits>
 
 #include "common.hpp"
