@@ -85,9 +85,10 @@ constexpr uint64_t kStreamBytes = 96ull << 20;
 constexpr uint32_t kPartKeysFew = 256, kPartKeysMany = 512, kManyPairs = 128;
 // Own keys in workgroups of 4 waves, four on a CU, where there are this many (row, KV head) pairs and none can have
 // more than kShortOwn own keys, by the caller's context_tokens: who passes the batch's longest length has this form,
-// who passes a capacity (a decode step, which also has at most 32 rows) the other one (160 rows of 8 KV heads with up to 300: 42.6 us, with 8 waves 47.6; 64 rows
-// with up to 60: 14.2, 15.3); a longest row sets the time else, and 8 waves are through with it
-// sooner (80 rows with up to 1500: 39.6 us, with 4 waves 44.5; 128 with 500 to 2000: 97.4, 102.6).
+// who passes a capacity (a decode step, which also has at most 32 rows) the other one (160 rows of 8 KV heads with up
+// to 300: 42.6 us, with 8 waves 47.6; 64 rows with up to 60: 14.2, 15.3). A longest row sets the time else, and 8
+// waves are through with it sooner (80 rows with up to 1500: 39.6 us, with 4 waves 44.5; 128 with 500 to 2000: 97.4,
+// 102.6).
 constexpr uint32_t kManyOwn = 512, kShortOwn = 512;
 constexpr uint32_t kMaxParts = 32;
 constexpr uint32_t kSlots = 512;      // workgroups that run at once: two on each CU

@@ -21,15 +21,13 @@ inline fh_status status_of(hipError_t e) {
   return FH_ERR_DEVICE;
 }
 
-// Launchers report hipGetLastError(), which also returns an error left
-// behind by an unrelated earlier runtime call on this thread; clear it first
-// so that the status belongs to this launch.
 inline bool aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
 // Head counts of the attention kernels and sizes whose products fit the launch.
 inline bool prefix_shape_ok(uint32_t rows, uint32_t qh, uint32_t kvh, uint32_t context) {
   // (A launch holds 2^32 threads: 512 a row and KV head.)
-  if (rows == 0 || rows > 65535u || kvh == 0 || kvh > 4096u || (uint64_t)rows * kvh > 1u << 22 || qh % kvh != 0 || context == 0 || context > 1u << 24)
+  if (rows == 0 || rows > 65535u || kvh == 0 || kvh > 4096u || (uint64_t)rows * kvh > 1u << 22 || qh % kvh != 0 ||
+      context == 0 || context > 1u << 24)
     return false;
   const uint32_t g = qh / kvh;
   return g == 1 || g == 2 || g == 4 || g == 8;
@@ -38,9 +36,13 @@ inline bool prefix_shape_ok(uint32_t rows, uint32_t qh, uint32_t kvh, uint32_t c
 // (A launch holds 2^32 threads: one for eight weights of the quantizer.)
 inline bool w4_size_ok(uint32_t n, uint32_t k) { return (uint64_t)n * k < 1ull << 35; }
 inline bool w4_shape_ok(uint32_t n, uint32_t k, uint32_t group) {
-  return n != 0 && k != 0 && n % 16 == 0 && k % 128 == 0 && k <= 1u << 24 && w4_size_ok(n, k) && (group == 32 || group == 64 || group == 128);
+  return n != 0 && k != 0 && n % 16 == 0 && k % 128 == 0 && k <= 1u << 24 && w4_size_ok(n, k) &&
+         (group == 32 || group == 64 || group == 128);
 }
 
+// Launchers report hipGetLastError(), which also returns an error left
+// behind by an unrelated earlier runtime call on this thread; clear it first
+// so that the status belongs to this launch.
 #define from_hip(expr) (static_cast<void>(hipGetLastError()), status_of(expr))
 
 }  // namespace
@@ -171,7 +173,8 @@ fh_status fh_op_gemm_w4(const uint16_t* x_tiled, const uint32_t* w_tiled, const 
     return FH_ERR_INVALID_ARGUMENT;
   if (!aligned(x_tiled, 16) || !aligned(w_tiled, 16) || !aligned(scales_tiled, 8) || !aligned(zeros_tiled, 4))
     return FH_ERR_INVALID_ARGUMENT;
-  if (epilogue > FH_EPI_PARTIAL || splits == 0 || splits > k / 128 || splits > 65535u || (epilogue != FH_EPI_PARTIAL && splits != 1) ||
+  if (epilogue > FH_EPI_PARTIAL || splits == 0 || splits > k / 128 || splits > 65535u ||
+      (epilogue != FH_EPI_PARTIAL && splits != 1) ||
       (epilogue == FH_EPI_RESIDUAL && !residual) || (epilogue == FH_EPI_SWIGLU ? n % 32 != 0 : ldo < n))
     return FH_ERR_INVALID_ARGUMENT;
   return from_hip(fh::launch_gemm_w4(x_tiled, w_tiled, scales_tiled, zeros_tiled, m, n, k, group, epilogue, splits,
