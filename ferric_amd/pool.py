@@ -328,7 +328,7 @@ class PagePool:
                 most = min(n, most, len(other))
                 differ = np.flatnonzero(pages[:most] != other[:most])
                 m = int(differ[0]) if len(differ) else most
-                if m < min_pages or rows * m < (rows - 1) * n:
+                if m < max(1, min_pages) or rows * m < (rows - 1) * n:
                     break
                 n, rows = m, rows + 1
             if rows > 1:

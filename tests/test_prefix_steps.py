@@ -130,3 +130,15 @@ def test_gains_of_several_groups_add_up_and_refused_groups_have_none():
         assert gain(bad, 32) == 0
     assert gain([(0, 32, 900)], 0) == 0 and gain([(0, 32, 900)], 32, heads=0) == 0 and gain([(0, 32, 0)], 32, context=0) == 0
     assert LIB.fh_prefix_groups_gain(None, 1, 32, 8, 16384) == 0
+
+
+@pytest.mark.parametrize("min_pages", [0, -3])
+def test_no_group_without_pages(min_pages):
+    """A step refuses a prefix of no pages, so none is listed."""
+    pool = PagePool(LIMITS, seed=6)
+    a, b = pool.admit(40), pool.admit(20)
+    c, _ = pool.fork(b)
+    batch = pool.prepare([(s, 1) for s in (a, b, c)])
+    assert PagePool.prefix_groups(batch, min_pages=min_pages) == [(1, 2, 1)]
+    d, e = pool.admit(0), pool.admit(5)
+    assert PagePool.prefix_groups(pool.prepare([(d, 1), (e, 1)]), min_pages=min_pages) == []
